@@ -11,6 +11,9 @@
 #include "kernels.h"
 #include "peer.h"
 
+// the residual layer's operators (bindings_res.cpp)
+void bind_residual(pybind11::module_& m);
+
 namespace d = grappa::dev;
 using at::Tensor;
 using OptT = std::optional<Tensor>;
@@ -1202,6 +1205,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("set_lr", &ArPlan::set_lr)
       .def("__len__", [](const ArPlan& p) { return p.args.size(); });
   m.doc() = "grappa_b200 sm_100a kernels";
+  bind_residual(m);
   m.def("sample_hop", &sample_hop, py::arg("indptr"), py::arg("indices"), py::arg("dst_nid"), py::arg("n_dst_dev"),
         py::arg("n_dst"), py::arg("frontier"), py::arg("fanout"), py::arg("replace"), py::arg("counters"),
         py::arg("hop"), py::arg("gideg"), py::arg("cov_accum"), py::arg("out_indptr"), py::arg("out_nbr"),

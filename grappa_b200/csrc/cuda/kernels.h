@@ -487,6 +487,160 @@ void launch_dropout_grad(float* g, int64_t ldg, int32_t dim, int64_t ld_mask, co
 void launch_f32_to_bf16_rows(float* src, int64_t lds, __nv_bfloat16* dst, int64_t ldd, int32_t dim,
                              const int32_t* n_ptr, int cap, bool clear, int32_t zero_tail_rows, cudaStream_t stream);
 
+// ---------------------------------------------------------------- residual layers
+// Rows in 8 bits (ckpt8.cuh): a row's columns in groups of 32; a group holds integer
+// codes of -127..127 and the exponent byte e of one power of two, 2^(e - 127), the
+// smallest with max|x| <= 127 * 2^(e-127) and e >= 1; a code c stands for c 2^(e-127).
+struct Rows8 {
+  int8_t* q = nullptr;      // [cap][ldq] codes, columns up to the next multiple of 32
+  int64_t ldq = 0;
+  uint8_t* e = nullptr;     // [cap][lde] exponent bytes, one per group
+  int64_t lde = 0;
+};
+
+// s = x + residual (rounded to the rows' type), rstd = 1 / sqrt(mean(s^2) + eps),
+// y = s rstd gamma; q8: the rows s rstd (before gamma) in 8 bits
+struct RmsNormArgs {
+  const void* x = nullptr;          // bf16 or fp32 rows
+  bool f32 = false;                 // type of x, residual and s_out
+  int64_t ldx = 0;
+  const void* residual = nullptr;
+  int64_t ldr = 0;
+  void* s_out = nullptr;
+  int64_t lds = 0;
+  int32_t dim = 0;                  // columns that count; outputs are zero up to the next multiple of 8
+  const int32_t* n_ptr = nullptr;
+  int32_t cap = 0;
+  const float* gamma = nullptr;     // [dim]
+  float eps = 1e-5f;
+  __nv_bfloat16* y = nullptr;
+  int64_t ldy = 0;
+  float* rstd = nullptr;            // [cap]
+  Rows8 q8;
+};
+void launch_rmsnorm_fwd(const RmsNormArgs& a, cudaStream_t stream);
+constexpr int kRmsNormMaxDim = 8192;
+
+// dx = rstd (gamma dy - xh mean(gamma dy xh)) + dres (rows below *n_res_ptr),
+// dgamma (+)= sum over the rows of dy xh; xh = x rstd, or the 8-bit rows
+struct RmsNormBwdArgs {
+  void* dy = nullptr;
+  bool dy_f32 = false;
+  int64_t lddy = 0;
+  bool clear_dy = false;            // zero dy after reading it
+  const void* x = nullptr;          // the rows that were normalised; null: q8
+  bool x_f32 = false;
+  int64_t ldx = 0;
+  Rows8 q8;
+  const float* rstd = nullptr;
+  const float* gamma = nullptr;
+  int32_t dim = 0;
+  const int32_t* n_ptr = nullptr;
+  int32_t cap = 0;
+  const void* dres = nullptr;
+  bool dres_f32 = false;
+  int64_t lddr = 0;
+  const int32_t* n_res_ptr = nullptr;  // rows that dres has (null: all of res_cap)
+  int32_t res_cap = 0;
+  void* dx = nullptr;
+  bool dx_f32 = false;
+  int64_t lddx = 0;
+  float* dgamma = nullptr;          // [dim]
+  bool accumulate = true;
+  float* work = nullptr;            // rmsnorm_bwd_work_floats() floats
+};
+int64_t rmsnorm_bwd_work_floats(int dim, int cap, int num_sms);
+void launch_rmsnorm_bwd(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream);
+
+// activations of the linear layer: 0 none, 1 ReLU, 2 GELU (tanh form), 3 SiLU
+enum LinearAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
+
+// out = dropout(act(z)) + residual, z = A W^T + bias; z kept as bf16 rows or in 8 bits
+struct LinearArgs {
+  const __nv_bfloat16* A = nullptr;  // [cap][lda]
+  int64_t a_rows = 0, lda = 0;
+  const __nv_bfloat16* W = nullptr;  // [N][ldw]
+  int64_t ldw = 0;
+  int32_t K = 0, N = 0;
+  const int32_t* n_ptr = nullptr;
+  int32_t cap = 0;
+  const float* bias = nullptr;       // [N]
+  int32_t act = kActNone;
+  float dropout_p = 0.f;
+  const int64_t* counters = nullptr;
+  uint32_t dropout_salt = 0;
+  const __nv_bfloat16* residual = nullptr;
+  int64_t r_rows = 0, ldr = 0;
+  __nv_bfloat16* out = nullptr;
+  int64_t out_rows = 0, ldo = 0;
+  __nv_bfloat16* z = nullptr;
+  int64_t ldz = 0;
+  Rows8 q8;
+  int64_t q_rows = 0;
+  int32_t* err = nullptr;
+};
+void launch_linear_fwd(const LinearArgs& a, cudaStream_t stream);
+
+// dz = dropout mask(dout) act'(z), dbias (+)= column sums of dz (before its rounding);
+// rows [n, roundup(n, 64)) of dz below cap are zeroed (the weight-gradient GEMM reads
+// whole 64-row blocks)
+struct LinearActBwdArgs {
+  void* dout = nullptr;
+  bool dout_f32 = false;
+  int64_t lddo = 0;
+  bool clear_dout = false;
+  const __nv_bfloat16* z = nullptr;
+  int64_t ldz = 0;
+  Rows8 q8;
+  int32_t dim = 0;
+  const int32_t* n_ptr = nullptr;
+  int32_t cap = 0;
+  int32_t act = kActNone;
+  float dropout_p = 0.f;
+  const int64_t* counters = nullptr;
+  uint32_t dropout_salt = 0;
+  int64_t ld_mask = 0;              // row stride that the forward drew its mask with
+  __nv_bfloat16* dz = nullptr;
+  int64_t lddz = 0;
+  float* dbias = nullptr;
+  bool accumulate = true;
+  float* work = nullptr;
+};
+int64_t linear_act_bwd_work_floats(int dim, int cap, int num_sms);
+void launch_linear_act_bwd(const LinearActBwdArgs& a, int num_sms, cudaStream_t stream);
+
+struct Ckpt8Args {
+  const void* x = nullptr;          // store: the rows; load: unused
+  void* out = nullptr;              // load: the rows that the codes stand for
+  bool f32 = false;
+  int64_t ld = 0;
+  int32_t dim = 0;
+  const int32_t* n_ptr = nullptr;
+  int32_t cap = 0;
+  Rows8 q8;
+};
+void launch_ckpt8_store(const Ckpt8Args& a, cudaStream_t stream);
+void launch_ckpt8_load(const Ckpt8Args& a, cudaStream_t stream);
+
+// gW[M][N] (+)= dY[:, :M]^T Xh[:, :N], Xh the rows that the codes stand for
+struct Ckpt8DwArgs {
+  const __nv_bfloat16* dy = nullptr;
+  int64_t dy_rows = 0, dy_cols = 0, lddy = 0;
+  Rows8 q8;
+  int64_t q_rows = 0, q_cols = 0;
+  int32_t groups = 0;               // exponent bytes a row
+  const int32_t* n_ptr = nullptr;
+  int32_t cap = 0;
+  float* gw = nullptr;
+  int64_t ldg = 0;
+  int32_t M = 0, N = 0;
+  bool accumulate = true;
+  float* work = nullptr;            // ckpt8_dw_work_floats() floats
+  int32_t* err = nullptr;
+};
+int64_t ckpt8_dw_work_floats(int M, int N, int cap, int num_sms);
+void launch_ckpt8_dw(const Ckpt8DwArgs& a, int num_sms, cudaStream_t stream);
+
 // ---------------------------------------------------------------- GAT (gat.cu)
 // Attention logits of every source row: el[u, h] = z_u[h] . a_l[h] and, for the
 // first n_dst rows, er[v, h] = z_v[h] . a_r[h] (z: bf16 [n_src, H*F]).

@@ -1,0 +1,379 @@
+// RMS norm of rows with the residual's addition, and its backward.
+//
+//   forward   s = x + r (rounded to the rows' type where it is written: the backward
+//             pass reads those rows), rstd = 1 / sqrt(mean_j s_j^2 + eps),
+//             y_j = s_j rstd gamma_j, and optionally xh_j = s_j rstd in 8 bits
+//   backward  dx_j = rstd (gamma_j dy_j - xh_j c) + dr_j,  c = mean_j gamma_j dy_j xh_j,
+//             dgamma_j = sum over the rows of dy_j xh_j
+//
+// Each row is read once and each output written once; a dozen operations an element, so
+// HBM bounds both.  A team of lanes holds a row in registers, eight columns (one or two
+// 16-byte loads) a lane and step: 4 to 32 lanes for rows of up to 32 * 8 columns, a warp
+// with up to four steps for up to 1024, a whole CTA above.  The row sums are shuffles (one
+// shared-memory exchange for CTA teams).  All sums and statistics are fp32.
+//
+// dgamma: a lane sums its columns over the rows of its team, the CTA joins its teams in
+// shared memory in a fixed order and writes one part, and a second kernel sums the parts
+// in order: the same bits every time, and no atomics.
+#include <algorithm>
+
+#include "ckpt8.cuh"
+#include "kernels.h"
+
+namespace grappa {
+namespace dev {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Eight columns of a row as they lie in memory, so that every load of a step is issued
+// before the first conversion: kind 0 bf16, 1 fp32, 2 codes.
+struct Raw8 {
+  uint4 a, b;
+};
+__device__ __forceinline__ Raw8 raw_load(const void* base, int64_t at, int kind) {
+  Raw8 r;
+  if (kind == 2) {
+    const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(base) + at);
+    r.a = make_uint4(q.x, q.y, 0u, 0u);
+  } else if (kind == 1) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + at);
+    r.a = p[0];
+    r.b = p[1];
+  } else {
+    r.a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at);
+  }
+  return r;
+}
+__device__ __forceinline__ void raw_values(const Raw8& r, int kind, float scale, float* v) {
+  if (kind == 2) {
+    values8(make_uint2(r.a.x, r.a.y), scale, v);
+  } else if (kind == 1) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+  } else {
+    bf16x8_to_f32(r.a, v);
+  }
+}
+__device__ __forceinline__ void store_any(void* base, int64_t at, bool f32, const float* v) {
+  if (f32)
+    store8(static_cast<float*>(base) + at, v);
+  else
+    store8(static_cast<__nv_bfloat16*>(base) + at, v);
+}
+
+// sum over the team of R values a lane; CTA teams exchange through sh[R][8]
+template <int TEAM, int R>
+__device__ __forceinline__ void team_sum(float (&s)[R], float (*sh)[8]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+  }
+  if constexpr (TEAM > 32) {
+    const int w = threadIdx.x >> 5;
+    __syncthreads();  // the last exchange has been read
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) sh[r][w] = s[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[r] += sh[r][i];
+    }
+  }
+}
+
+template <int TEAM, int NV, int R>
+__global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
+  GB_PDL_ENTRY();
+  __shared__ float sh[R][8];
+  constexpr int kTeams = kThreads / TEAM;
+  const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const int n = live_rows(a.n_ptr, a.cap);
+  const int kind = a.f32 ? 1 : 0;
+  const int chunks = (a.dim + 7) / 8;
+  const int qchunks = a.q8.q ? (a.dim + 31) / 32 * 4 : chunks;
+  const float inv_dim = 1.f / static_cast<float>(a.dim);
+  // a CTA takes kTeams * R consecutive rows at a time (uniform trip count per warp)
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * R; base < n;
+       base += static_cast<int64_t>(gridDim.x) * kTeams * R) {
+    Raw8 raw[R][NV], rr[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * kTeams + team;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TEAM + t;
+        const bool on = row < n && c < chunks;
+        raw[r][i].a = raw[r][i].b = rr[r][i].a = rr[r][i].b = make_uint4(0u, 0u, 0u, 0u);
+        if (on) raw[r][i] = raw_load(a.x, row * a.ldx + c * 8, kind);
+        if (on && a.residual) rr[r][i] = raw_load(a.residual, row * a.ldr + c * 8, kind);
+      }
+    }
+    float v[R][NV][8], ss[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      ss[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TEAM + t;
+        raw_values(raw[r][i], kind, 0.f, v[r][i]);
+        if (a.residual) {
+          float w[8];
+          raw_values(rr[r][i], kind, 0.f, w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[r][i][j] += w[j];
+            if (!a.f32) v[r][i][j] = __bfloat162float(__float2bfloat16_rn(v[r][i][j]));
+          }
+        }
+        mask8(v[r][i], c, a.dim);
+        if (a.s_out && row < n && c < chunks) store_any(a.s_out, row * a.lds + c * 8, a.f32, v[r][i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss[r] = fmaf(v[r][i][j] * inv_dim, v[r][i][j], ss[r]);
+      }
+    }
+    team_sum<TEAM, R>(ss, sh);  // the mean: each term is divided, so that it fits fp32 where the mean does
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      const float rs = 1.f / sqrtf(ss[r] + a.eps);
+      if (t == 0 && row < n) a.rstd[row] = rs;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TEAM + t;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[r][i][j] *= rs;
+          y[j] = c * 8 + j < a.dim ? v[r][i][j] * __ldg(a.gamma + c * 8 + j) : 0.f;
+        }
+        if (row < n && c < chunks) store8(a.y + row * a.ldy + c * 8, y);
+        if (a.q8.q) {
+          uint32_t m = abs_max_bits8(v[r][i]);
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const uint32_t byte = group8_byte(m);
+          if (row < n && c < qchunks) {
+            *reinterpret_cast<uint2*>(a.q8.q + row * a.q8.ldq + c * 8) = codes8(v[r][i], group8_inv(byte));
+            if ((c & 3) == 0) a.q8.e[row * a.q8.lde + (c >> 2)] = static_cast<uint8_t>(byte);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <int TEAM, int NV, int R>
+__global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a) {
+  GB_PDL_ENTRY();
+  __shared__ float sh[R][8];
+  extern __shared__ float parts[];  // [kTeams][TEAM * NV * 8]
+  constexpr int kTeams = kThreads / TEAM;
+  constexpr int kCols = TEAM * NV * 8;
+  const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const int n = live_rows(a.n_ptr, a.cap);
+  const int n_res = a.dres ? min(live_rows(a.n_res_ptr, a.res_cap), n) : 0;
+  const int ydk = a.dy_f32 ? 1 : 0, xk = a.x ? (a.x_f32 ? 1 : 0) : 2, rk = a.dres_f32 ? 1 : 0;
+  const int chunks = (a.dim + 7) / 8;
+  const float inv_dim = 1.f / static_cast<float>(a.dim);
+  float acc[NV][8], gam[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int col = (i * TEAM + t) * 8 + j;
+      acc[i][j] = 0.f;
+      gam[i][j] = col < a.dim ? a.gamma[col] : 0.f;
+    }
+  }
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * R; base < n;
+       base += static_cast<int64_t>(gridDim.x) * kTeams * R) {
+    Raw8 yr[R][NV], xr[R][NV], rr[R][NV];
+    uint32_t eb[R][NV];
+    float rs[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      rs[r] = row < n ? a.rstd[row] : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TEAM + t;
+        yr[r][i].a = yr[r][i].b = xr[r][i].a = xr[r][i].b = rr[r][i].a = rr[r][i].b = make_uint4(0u, 0u, 0u, 0u);
+        eb[r][i] = 0;
+        if (row < n && c < chunks) {
+          yr[r][i] = raw_load(a.dy, row * a.lddy + c * 8, ydk);
+          if (xk == 2) {
+            xr[r][i] = raw_load(a.q8.q, row * a.q8.ldq + c * 8, 2);
+            eb[r][i] = a.q8.e[row * a.q8.lde + (c >> 2)];
+          } else {
+            xr[r][i] = raw_load(a.x, row * a.ldx + c * 8, xk);
+          }
+          if (row < n_res) rr[r][i] = raw_load(a.dres, row * a.lddr + c * 8, rk);
+        }
+      }
+    }
+    float dy[R][NV][8], xh[R][NV][8], dot[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      dot[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TEAM + t;
+        raw_values(yr[r][i], ydk, 0.f, dy[r][i]);
+        raw_values(xr[r][i], xk, group8_scale(eb[r][i]), xh[r][i]);
+        mask8(dy[r][i], c, a.dim);
+        mask8(xh[r][i], c, a.dim);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (xk != 2) xh[r][i][j] *= rs[r];
+          const float p = dy[r][i][j] * xh[r][i][j];
+          acc[i][j] += p;
+          dot[r] = fmaf(p, gam[i][j], dot[r]);
+        }
+      }
+    }
+    team_sum<TEAM, R>(dot, sh);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      const float mean = dot[r] * inv_dim;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TEAM + t;
+        if (row < n && c < chunks) {
+          float dr[8], o[8];
+          raw_values(rr[r][i], rk, 0.f, dr);
+          mask8(dr, c, a.dim);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            o[j] = fmaf(rs[r], fmaf(-xh[r][i][j], mean, gam[i][j] * dy[r][i][j]), dr[j]);
+          if (a.clear_dy) {
+            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            store_any(a.dy, row * a.lddy + c * 8, a.dy_f32, z);
+          }
+          store_any(a.dx, row * a.lddx + c * 8, a.dx_f32, o);
+        }
+      }
+    }
+  }
+  // the CTA's part of dgamma: its teams in order
+  float* out = a.work + static_cast<int64_t>(blockIdx.x) * a.dim;
+  if constexpr (kTeams == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((i * TEAM + t) * 8 + j < a.dim) out[(i * TEAM + t) * 8 + j] = acc[i][j];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) parts[team * kCols + (i * TEAM + t) * 8 + j] = acc[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+      float s = 0.f;
+#pragma unroll 8
+      for (int p = 0; p < kTeams; ++p) s += parts[p * kCols + c];
+      out[c] = s;
+    }
+  }
+}
+
+// one CTA per 32 columns; 32 threads a column, each a strided share of the parts
+__global__ void __launch_bounds__(1024)
+    sum_parts_kernel(const float* part, int parts, int64_t ld, int cols, float* out, bool accumulate) {
+  GB_PDL_ENTRY();
+  __shared__ float sh[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 4
+    for (int p = threadIdx.y; p < parts; p += 32) s += part[p * ld + c];
+  }
+  sh[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+    float v = accumulate ? out[c] : 0.f;
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w += sh[i][threadIdx.x];
+    out[c] = v + w;
+  }
+}
+
+// rows a CTA takes at a time, and the CTAs for cap rows: all of them at once up to
+// kCtasPerSm on every SM
+constexpr int kCtasPerSm = 4;
+template <int TEAM, int R>
+int grid_rows(int cap, int num_sms) {
+  return static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>(ceil_div(cap, kThreads / TEAM * R), static_cast<int64_t>(num_sms) * kCtasPerSm)));
+}
+
+template <int TEAM, int NV, int R>
+void fwd_t(const RmsNormArgs& a, cudaStream_t stream) {
+  // not persistent: one pass of rows a CTA, the hardware refills the SMs
+  const int64_t grid = ceil_div(a.cap, kThreads / TEAM * R);
+  launch_k(rmsnorm_fwd_kernel<TEAM, NV, R>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+  GB_LAUNCH_CHECK();
+}
+
+template <int TEAM, int NV, int R>
+void bwd_t(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
+  const int grid = grid_rows<TEAM, R>(a.cap, num_sms);
+  const size_t smem = TEAM < kThreads ? sizeof(float) * kThreads * NV * 8 : 0;
+  launch_k(rmsnorm_bwd_kernel<TEAM, NV, R>, dim3(grid), dim3(kThreads), smem, stream, a);
+  GB_LAUNCH_CHECK();
+  launch_sum_parts(a.work, grid, a.dim, a.dim, a.dgamma, a.accumulate, stream);
+}
+
+}  // namespace
+
+void launch_sum_parts(const float* part, int parts, int64_t ld, int cols, float* out, bool accumulate,
+                      cudaStream_t stream) {
+  launch_k(sum_parts_kernel, dim3(static_cast<unsigned>(ceil_div(cols, 32))), dim3(32, 32), 0, stream, part, parts, ld,
+           cols, out, accumulate);
+  GB_LAUNCH_CHECK();
+}
+
+int64_t rmsnorm_bwd_work_floats(int dim, int cap, int num_sms) {
+  return static_cast<int64_t>(dim) * std::min<int64_t>(std::max(cap, 1), static_cast<int64_t>(num_sms) * kCtasPerSm);
+}
+
+void launch_rmsnorm_fwd(const RmsNormArgs& a, cudaStream_t stream) {
+  if (a.cap <= 0) return;
+  const int d = a.dim;
+  if (d <= 32) return fwd_t<4, 1, 2>(a, stream);
+  if (d <= 64) return fwd_t<8, 1, 2>(a, stream);
+  if (d <= 128) return fwd_t<16, 1, 2>(a, stream);
+  if (d <= 256) return fwd_t<32, 1, 2>(a, stream);
+  if (d <= 512) return fwd_t<32, 2, 1>(a, stream);
+  if (d <= 1024) return fwd_t<32, 4, 1>(a, stream);
+  if (d <= 2048) return fwd_t<256, 1, 2>(a, stream);
+  if (d <= 4096) return fwd_t<256, 2, 1>(a, stream);
+  return fwd_t<256, 4, 1>(a, stream);
+}
+
+void launch_rmsnorm_bwd(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
+  const int d = a.dim;
+  if (d <= 32) return bwd_t<4, 1, 2>(a, num_sms, stream);
+  if (d <= 64) return bwd_t<8, 1, 2>(a, num_sms, stream);
+  if (d <= 128) return bwd_t<16, 1, 2>(a, num_sms, stream);
+  if (d <= 256) return bwd_t<32, 1, 2>(a, num_sms, stream);
+  if (d <= 512) return bwd_t<32, 2, 1>(a, num_sms, stream);
+  if (d <= 1024) return bwd_t<32, 4, 1>(a, num_sms, stream);
+  if (d <= 2048) return bwd_t<256, 1, 2>(a, num_sms, stream);
+  if (d <= 4096) return bwd_t<256, 2, 1>(a, num_sms, stream);
+  return bwd_t<256, 4, 1>(a, num_sms, stream);
+}
+
+}  // namespace dev
+}  // namespace grappa

@@ -92,7 +92,8 @@ KERNELS_PER_CALL = {
     "gat_scores": 1, "gat_fwd": 1, "gat_bwd": 2, "gat_bwd_input": 2, "gat_dw_combine": 1, "sampler_counters": 1,
     "gat_in_scores": 1, "gat_in_fwd": 1, "gat_in_bwd": 2, "gat_in_prep": 1, "gat_in_dw": 1, "col_sum_bf16": 1,
     "block_transpose": 2, "aggregate_bwd_gather": 1, "sage_head": 1, "compact_edges": 1, "sage_layer_fwd": 1,
-    "sage_layer_bwd": 1,
+    "sage_layer_bwd": 1, "rmsnorm_fwd": 1, "rmsnorm_bwd": 2, "linear_fwd": 1, "linear_act_bwd": 2, "ckpt8_store": 1,
+    "ckpt8_load": 1, "ckpt8_dw": 2,
 }
 
 
