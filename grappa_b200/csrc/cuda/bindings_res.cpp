@@ -198,7 +198,7 @@ void rmsnorm_fwd(Tensor x, int64_t dim, OptT n_dev, int64_t cap, Tensor gamma, d
   a.n_ptr = count(n_dev, "n_dev");
   const auto dev = on_device({&x, &gamma, &y, &rstd}, {&n_dev, &residual, &s_out, &q, &q_exp});
   c10::cuda::CUDAGuard g(dev);
-  d::launch_rmsnorm_fwd(a, stream());
+  d::launch_rmsnorm_fwd(a, sms(), stream());
 }
 
 void rmsnorm_bwd(Tensor dy, OptT x, Tensor rstd, Tensor gamma, int64_t dim, OptT n_dev, int64_t cap, Tensor dx,
@@ -227,9 +227,8 @@ void rmsnorm_bwd(Tensor dy, OptT x, Tensor rstd, Tensor gamma, int64_t dim, OptT
   a.n_res_ptr = count(n_res_dev, "n_res_dev");
   if (has(dres)) {
     // with a row count of its own it may have fewer rows (the kernel reads below both counts)
-    mr = mat(*dres, "dres", {at::kBFloat16, at::kFloat}, a.n_res_ptr ? 0 : cap, w, kRead);
+    mr = mat(*dres, "dres", {dx.scalar_type()}, a.n_res_ptr ? 0 : cap, w, kRead);
     a.dres = mr.p;
-    a.dres_f32 = f32(*dres);
     a.lddr = mr.ld;
     a.res_cap = static_cast<int32_t>(std::min<int64_t>(mr.rows, cap));
   }
@@ -296,7 +295,6 @@ void linear_fwd(Tensor A, Tensor W, OptT n_dev, int64_t cap, Tensor out, Tensor 
   }
   std::vector<Mat> coded;
   a.q8 = rows8(q, q_exp, cap, N, kWrite, &coded);
-  if (!coded.empty()) a.q_rows = coded[0].rows;
   for (const Mat& m : coded) {
     all_apart(m, others);
     apart(m, mr);
@@ -453,8 +451,8 @@ not read and are written as zeros.  s_out may be x or residual itself.  dim <= 8
 
 dx = rstd (gamma dy - xh mean(gamma dy xh)) + dres,  dgamma (+)= sum over the rows of dy xh
 (+= unless accumulate is False), with xh = x rstd (x: the rows that were normalised, s_out
-where there was a residual) or, with x None, the 8-bit rows q / q_exp.  dy, x, dres and dx are
-bf16 or float32 each.  dres (the gradient that reaches the residual stream from above) has
+where there was a residual) or, with x None, the 8-bit rows q / q_exp.  dy, x and dx are
+bf16 or float32 each, dres as dx.  dres (the gradient that reaches the residual stream from above) has
 min(*n_res_dev, n) rows when n_res_dev is given; rows past them get none.  clear_dy zeroes
 dy after reading it.  dx may be dres, or dy without clear_dy.  dgamma has the same bits on
 every run.)");

@@ -2,14 +2,15 @@
 //
 // All three are one pass over their rows with a few operations an element (the
 // activation's slope: an exponential and a division), so HBM bounds them.  A lane takes
-// eight columns (16 bytes of bf16) of a row; four neighbouring lanes hold a group of 32
-// and find its largest magnitude with two shuffles.
+// sixteen columns of a row (eight in the activation backward), and several rows in flight.
 #include <algorithm>
+#include <type_traits>
 
 #include "ckpt8.cuh"
 #include "grappa/rng.h"
 #include "kernels.h"
 #include "linear_act.cuh"
+#include "tcgen05.cuh"
 
 namespace grappa {
 namespace dev {
@@ -17,90 +18,118 @@ namespace dev {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // chunks a thread has in flight
+constexpr int kRowsC = 2;  // rows a thread has in flight
 
-// A CTA takes kThreads * kUnroll chunks of consecutive rows; chunk i of the tile is column
-// chunk i % cpr of row i / cpr (cpr: chunks of a row up to the next group, a multiple of 4,
-// so a group never straddles two rows and its four chunks are four neighbouring lanes).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) ckpt8_store_kernel(Ckpt8Args a) {
+// LPR lanes x 16 columns cover a row (blockIdx.y the next LPR * 16 columns of wide rows);
+// lanes 2i and 2i + 1 hold a group.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kThreads, 4) ckpt8_store_kernel(Ckpt8Args a) {
   GB_PDL_ENTRY();
+  constexpr int kTeams = kThreads / LPR;
   const int n = live_rows(a.n_ptr, a.cap);
-  const uint32_t cpr = static_cast<uint32_t>((a.dim + 31) / 32 * 4);
-  const int64_t total = static_cast<int64_t>(n) * cpr;
-  const int64_t tile0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kUnroll);
-  if (tile0 >= total) return;
-  const int64_t row0 = tile0 / cpr;
-  const uint32_t off0 = static_cast<uint32_t>(tile0 - row0 * cpr);
-  float v[kUnroll][8];
-  int64_t row[kUnroll];
-  uint32_t c[kUnroll];
-  bool live[kUnroll];
+  const int t = threadIdx.x % LPR, team = threadIdx.x / LPR;
+  const int c = (blockIdx.y * LPR + t) * 16;  // first column
+  const bool in = c < (a.dim + 31) / 32 * 32;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * kRowsC; base < n;
+       base += static_cast<int64_t>(gridDim.x) * kTeams * kRowsC) {
+    float v[kRowsC][16];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const uint32_t i = off0 + u * kThreads + threadIdx.x;
-    row[u] = row0 + i / cpr;
-    c[u] = i % cpr;
-    live[u] = row[u] < n;
+    for (int r = 0; r < kRowsC; ++r) {
+      const int64_t row = base + r * kTeams + team;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-    if (live[u] && c[u] * 8 < static_cast<uint32_t>(a.dim)) load8(static_cast<const T*>(a.x) + row[u] * a.ld + c[u] * 8, v[u]);
-  }
+      for (int j = 0; j < 16; ++j) v[r][j] = 0.f;
+      const T* p = static_cast<const T*>(a.x) + row * a.ld + c;
+      if (row < n && c < a.dim) load8(p, v[r]);
+      if (row < n && c + 8 < a.dim) load8(p + 8, v[r] + 8);
+    }
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    mask8(v[u], static_cast<int>(c[u]), a.dim);
-    uint32_t m = abs_max_bits8(v[u]);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t byte = group8_byte(m);
-    if (live[u]) {
-      *reinterpret_cast<uint2*>(a.q8.q + row[u] * a.q8.ldq + c[u] * 8) = codes8(v[u], group8_inv(byte));
-      if ((c[u] & 3u) == 0) a.q8.e[row[u] * a.q8.lde + (c[u] >> 2)] = static_cast<uint8_t>(byte);
+    for (int r = 0; r < kRowsC; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      mask8(v[r], c >> 3, a.dim);
+      mask8(v[r] + 8, (c >> 3) + 1, a.dim);
+      float m = max_nan(abs_max8(v[r]), abs_max8(v[r] + 8));
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      const uint32_t byte = group8_byte(m);
+      const float inv = group8_inv(byte);
+      if (row < n && in) {
+        const uint2 q0 = codes8(v[r], inv), q1 = codes8(v[r] + 8, inv);
+        *reinterpret_cast<uint4*>(a.q8.q + row * a.q8.ldq + c) = make_uint4(q0.x, q0.y, q1.x, q1.y);
+        if ((t & 1) == 0) a.q8.e[row * a.q8.lde + (c >> 5)] = static_cast<uint8_t>(byte);
+      }
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) ckpt8_load_kernel(Ckpt8Args a) {
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kThreads, 4) ckpt8_load_kernel(Ckpt8Args a) {
   GB_PDL_ENTRY();
+  constexpr int kTeams = kThreads / LPR;
   const int n = live_rows(a.n_ptr, a.cap);
-  const uint32_t cpr = static_cast<uint32_t>((a.dim + 7) / 8);
-  const int64_t total = static_cast<int64_t>(n) * cpr;
-  const int64_t tile0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kUnroll);
-  if (tile0 >= total) return;
-  const int64_t row0 = tile0 / cpr;
-  const uint32_t off0 = static_cast<uint32_t>(tile0 - row0 * cpr);
-  uint2 q[kUnroll];
-  uint32_t e[kUnroll], c[kUnroll];
-  int64_t row[kUnroll];
+  const int t = threadIdx.x % LPR, team = threadIdx.x / LPR;
+  const int c = (blockIdx.y * LPR + t) * 16;
+  if (c >= a.dim) return;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * kRowsC; base < n;
+       base += static_cast<int64_t>(gridDim.x) * kTeams * kRowsC) {
+    uint4 q[kRowsC];
+    uint32_t e[kRowsC];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const uint32_t i = off0 + u * kThreads + threadIdx.x;
-    row[u] = row0 + i / cpr;
-    c[u] = i % cpr;
-    q[u] = make_uint2(0u, 0u);
-    e[u] = 0;
-    if (row[u] < n) {
-      q[u] = *reinterpret_cast<const uint2*>(a.q8.q + row[u] * a.q8.ldq + c[u] * 8);
-      e[u] = a.q8.e[row[u] * a.q8.lde + (c[u] >> 2)];
+    for (int r = 0; r < kRowsC; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      q[r] = make_uint4(0u, 0u, 0u, 0u);
+      e[r] = 0u;
+      if (row < n) {
+        q[r] = *reinterpret_cast<const uint4*>(a.q8.q + row * a.q8.ldq + c);
+        e[r] = a.q8.e[row * a.q8.lde + (c >> 5)];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRowsC; ++r) {
+      const int64_t row = base + r * kTeams + team;
+      if (row >= n) continue;
+      T* p = static_cast<T*>(a.out) + row * a.ld + c;
+      if (sizeof(T) == 2 && c + 16 <= a.dim) {
+        const __nv_bfloat162 scale = group8_scale_bf16(e[r]);
+        *reinterpret_cast<uint4*>(p) = values8_bf16(q[r].x, q[r].y, scale);
+        *reinterpret_cast<uint4*>(p + 8) = values8_bf16(q[r].z, q[r].w, scale);
+      } else {
+        float v[8];
+        values8(make_uint2(q[r].x, q[r].y), group8_scale(e[r]), v);
+        mask8(v, c >> 3, a.dim);
+        store8(p, v);
+        if (c + 8 < a.dim) {
+          values8(make_uint2(q[r].z, q[r].w), group8_scale(e[r]), v);
+          mask8(v, (c >> 3) + 1, a.dim);
+          store8(p + 8, v);
+        }
+      }
     }
   }
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    float v[8];
-    values8(q[u], group8_scale(e[u]), v);
-    mask8(v, static_cast<int>(c[u]), a.dim);
-    if (row[u] < n) store8(static_cast<T*>(a.out) + row[u] * a.ld + c[u] * 8, v);
-  }
+}
+
+// calls f with the lanes per row (a compile-time constant) for rows of `dim` columns
+template <typename F>
+void with_lpr(int dim, F&& f) {
+  if (dim <= 32) return f(std::integral_constant<int, 2>());
+  if (dim <= 64) return f(std::integral_constant<int, 4>());
+  if (dim <= 128) return f(std::integral_constant<int, 8>());
+  if (dim <= 256) return f(std::integral_constant<int, 16>());
+  return f(std::integral_constant<int, 32>());
+}
+template <int LPR>
+dim3 ckpt_grid(int dim, int cap) {
+  // as many CTAs as the SMs hold at once: short-lived ones measured a third slower
+  const int64_t passes = ceil_div(cap, kThreads / LPR * kRowsC), slices = ceil_div(ceil_div(dim, 32) * 2, LPR);
+  return dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(passes, ceil_div(sm_count() * 4, slices)))),
+              static_cast<unsigned>(slices));
 }
 
 // dz = mask(dout) act'(z): a warp takes LPR lanes x 8 columns of 32 / LPR rows, kRows of
 // them in flight; blockIdx.y walks the 256-column slices of wide rows.  The column sums go
 // through shared memory into one part a CTA, as in the norm's backward.
-constexpr int kRows = 4;
+constexpr int kRows = 1;
 
 template <int LPR, bool F32, bool Q8>
-__global__ void __launch_bounds__(kThreads) linear_act_bwd_kernel(LinearActBwdArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) linear_act_bwd_kernel(LinearActBwdArgs a) {
   GB_PDL_ENTRY();
   constexpr int kTeams = kThreads / LPR;
   __shared__ float parts[kTeams][LPR * 8];
@@ -160,17 +189,19 @@ __global__ void __launch_bounds__(kThreads) linear_act_bwd_kernel(LinearActBwdAr
         values8(make_uint2(zr[r].x, zr[r].y), group8_scale(eb[r]), z);
       else
         bf16x8_to_f32(zr[r], z);
-      mask8(g, c, a.dim);
-      mask8(z, c, a.dim);
+      if (c * 8 + 8 > a.dim) {
+        mask8(g, c, a.dim);
+        mask8(z, c, a.dim);
+      }
       if (a.act == kActRelu) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = z[j] > 0.f ? g[j] : 0.f;
       } else if (a.act == kActGelu) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= gelu_slope(z[j]);
+        for (int j = 0; j < 8; j += 2) gelu_slope2(z + j, g + j);
       } else if (a.act == kActSilu) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= silu_slope(z[j]);
+        for (int j = 0; j < 8; j += 2) silu_slope2(z + j, g + j);
       }
       if (a.dropout_p > 0.f) {
         const uint64_t at = static_cast<uint64_t>(row) * static_cast<uint64_t>(a.ld_mask) + static_cast<uint64_t>(c) * 8;
@@ -208,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) linear_act_bwd_kernel(LinearActBwdAr
   }
 }
 
-constexpr int kCtasPerSm = 8;
+constexpr int kCtasPerSm = 4;
 
 int act_bwd_grid(int dim, int cap, int num_sms) {
   const int lpr = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
@@ -248,17 +279,21 @@ void launch_linear_act_bwd(const LinearActBwdArgs& a, int num_sms, cudaStream_t 
 
 void launch_ckpt8_store(const Ckpt8Args& a, cudaStream_t stream) {
   if (a.cap <= 0) return;
-  const int64_t grid = ceil_div(static_cast<int64_t>(a.cap) * ceil_div(a.dim, 32) * 4, kThreads * kUnroll);
-  launch_k(a.f32 ? ckpt8_store_kernel<float> : ckpt8_store_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(grid)),
-           dim3(kThreads), 0, stream, a);
+  with_lpr(a.dim, [&](auto lpr) {
+    constexpr int L = decltype(lpr)::value;
+    launch_k(a.f32 ? ckpt8_store_kernel<float, L> : ckpt8_store_kernel<__nv_bfloat16, L>, ckpt_grid<L>(a.dim, a.cap),
+             dim3(kThreads), 0, stream, a);
+  });
   GB_LAUNCH_CHECK();
 }
 
 void launch_ckpt8_load(const Ckpt8Args& a, cudaStream_t stream) {
   if (a.cap <= 0) return;
-  const int64_t grid = ceil_div(static_cast<int64_t>(a.cap) * ceil_div(a.dim, 8), kThreads * kUnroll);
-  launch_k(a.f32 ? ckpt8_load_kernel<float> : ckpt8_load_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(grid)),
-           dim3(kThreads), 0, stream, a);
+  with_lpr(a.dim, [&](auto lpr) {
+    constexpr int L = decltype(lpr)::value;
+    launch_k(a.f32 ? ckpt8_load_kernel<float, L> : ckpt8_load_kernel<__nv_bfloat16, L>, ckpt_grid<L>(a.dim, a.cap),
+             dim3(kThreads), 0, stream, a);
+  });
   GB_LAUNCH_CHECK();
 }
 

@@ -10,15 +10,16 @@
 // of it reads back as NaN.  The byte 0 (a cleared buffer) stands for zeros.
 #pragma once
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace grappa {
 namespace dev {
 
 constexpr int kGroup8 = 32;
 
-// Exponent byte of a group from the largest |x| bit pattern in it (integer order of the
-// patterns of non-negative floats is their order, with infinities and NaN above all).
-__device__ __forceinline__ uint32_t group8_byte(uint32_t abs_bits) {
+// Exponent byte of a group from its largest |x| (NaN if it holds one).
+__device__ __forceinline__ uint32_t group8_byte(float top) {
+  const uint32_t abs_bits = __float_as_uint(top);
   if (abs_bits >= 0x7F800000u) return 255u;
   // |x| = m 2^k, 1 <= m < 2: 127 * 2^E >= |x| first at E = k - 6 while 64 m <= 127
   const uint32_t over = (abs_bits & 0x7FFFFFu) > 0x7E0000u ? 1u : 0u;
@@ -32,35 +33,73 @@ __device__ __forceinline__ float group8_inv(uint32_t byte) {
 // 2^E; infinity for the byte 255 (0 * infinity = NaN), 0 for the byte 0
 __device__ __forceinline__ float group8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// x 2^-E rounded to the nearest integer, ties to even, in the low byte.  |x 2^-E| <= 127,
-// so adding 1.5 * 2^23 rounds at the unit and leaves the integer in the low mantissa bits.
-__device__ __forceinline__ uint32_t code8(float x, float inv) {
-  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)) & 0xFFu;
-}
+// x 2^-E rounded to the nearest integer, ties to even, in the low byte.  |x 2^-E| <= 127 and
+// the product is exact, so adding 1.5 * 2^23 in the same operation rounds at the unit and
+// leaves the integer in the low mantissa bits.
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-// eight codes of one chunk (a group's columns are four consecutive chunks)
+// eight codes of one chunk (a group's columns are four consecutive chunks); inv = 0, of a
+// group that is not finite, makes codes 0 of its finite values, and the others are masked
 __device__ __forceinline__ uint2 codes8(const float* v, float inv) {
-  if (inv == 0.f) return make_uint2(0u, 0u);
   uint32_t c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = code8(v[i], inv);
-  return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-}
-__device__ __forceinline__ uint32_t abs_max_bits8(const float* v) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return m;
-}
-// the eight values of a chunk's codes
-__device__ __forceinline__ void values8(uint2 q, float scale, float* v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = static_cast<float>(static_cast<int8_t>(q.x >> (8 * i))) * scale;
-    v[4 + i] = static_cast<float>(static_cast<int8_t>(q.y >> (8 * i))) * scale;
+  for (int i = 0; i < 8; i += 2) {
+    float a, b;
+    unpack(fma2(f2(v[i], v[i + 1]), both(inv), both(12582912.f)), a, b);
+    c[i] = __float_as_uint(a), c[i + 1] = __float_as_uint(b);
   }
+  const uint32_t on = inv == 0.f ? 0u : 0xFFFFFFFFu;
+  return make_uint2(pack4(c[0], c[1], c[2], c[3]) & on, pack4(c[4], c[5], c[6], c[7]) & on);
+}
+// max(|a|, |b|, |c|), NaN if one of them is
+__device__ __forceinline__ float abs_max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float abs_max8(const float* v) {
+  return max_nan(abs_max3(abs_max3(v[0], v[1], v[2]), v[3], v[4]), abs_max3(v[5], v[6], v[7]));
+}
+// the eight values of a chunk's codes: a code c + 128 in the low byte of 2^23 is the float
+// 8388736 + c (a byte permutation instead of the quarter-rate integer conversion)
+__device__ __forceinline__ void values8(uint2 q, float scale, float* v) {
+  q.x ^= 0x80808080u;
+  q.y ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint32_t w = i < 4 ? q.x : q.y;
+    const F2 c = f2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + (i & 3))),
+                    __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7541 + (i & 3))));
+    unpack(mul2(add2(c, both(-8388736.f)), both(scale)), v[i], v[i + 1]);
+  }
+}
+// The same as four bf16 pairs, without passing through fp32: with x = c + 128 = 128 h + m (m of
+// seven bits), c = (128 + m) - (256 - 128 h); both terms are bf16 patterns made by one logic
+// operation a pair (0x4300 | m, and 0x4380 with the bit h cleared from its exponent), their
+// difference and its product with the power of two are exact.
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t x, uint32_t sel, __nv_bfloat162 scale) {
+  const uint32_t p = __byte_perm(x, 0u, sel);
+  const uint32_t a = (p & 0x007F007Fu) | 0x43004300u, b = (p & 0x00800080u) ^ 0x43804380u;
+  const __nv_bfloat162 d = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                           *reinterpret_cast<const __nv_bfloat162*>(&b)), scale);
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint4 values8_bf16(uint32_t qx, uint32_t qy, __nv_bfloat162 scale) {
+  qx ^= 0x80808080u;
+  qy ^= 0x80808080u;
+  return make_uint4(pair_bf16(qx, 0x4140, scale), pair_bf16(qx, 0x4342, scale), pair_bf16(qy, 0x4140, scale),
+                    pair_bf16(qy, 0x4342, scale));
+}
+// 2^E as a bf16 pair (the byte is the exponent field)
+__device__ __forceinline__ __nv_bfloat162 group8_scale_bf16(uint32_t byte) {
+  const uint32_t s = byte * 0x00800080u;
+  return *reinterpret_cast<const __nv_bfloat162*>(&s);
 }
 
 // Eight consecutive columns of a bf16 or fp32 row (16-byte aligned), as fp32 and back.

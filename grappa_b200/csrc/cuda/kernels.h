@@ -518,7 +518,7 @@ struct RmsNormArgs {
   float* rstd = nullptr;            // [cap]
   Rows8 q8;
 };
-void launch_rmsnorm_fwd(const RmsNormArgs& a, cudaStream_t stream);
+void launch_rmsnorm_fwd(const RmsNormArgs& a, int num_sms, cudaStream_t stream);
 constexpr int kRmsNormMaxDim = 8192;
 
 // dx = rstd (gamma dy - xh mean(gamma dy xh)) + dres (rows below *n_res_ptr),
@@ -537,8 +537,7 @@ struct RmsNormBwdArgs {
   int32_t dim = 0;
   const int32_t* n_ptr = nullptr;
   int32_t cap = 0;
-  const void* dres = nullptr;
-  bool dres_f32 = false;
+  const void* dres = nullptr;       // type of dx
   int64_t lddr = 0;
   const int32_t* n_res_ptr = nullptr;  // rows that dres has (null: all of res_cap)
   int32_t res_cap = 0;
@@ -576,7 +575,6 @@ struct LinearArgs {
   __nv_bfloat16* z = nullptr;
   int64_t ldz = 0;
   Rows8 q8;
-  int64_t q_rows = 0;
   int32_t* err = nullptr;
 };
 void launch_linear_fwd(const LinearArgs& a, cudaStream_t stream);

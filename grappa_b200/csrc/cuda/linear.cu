@@ -8,11 +8,10 @@
 //               128B-swizzled buffers that runs across tiles)
 //   warp 1      issues tcgen05.mma (M = 128, N = BN, K = 16) into one of two TMEM
 //               accumulators, so the epilogue of a tile overlaps the products of the next
-//   warps 2..   epilogue: each warp owns 32 rows (a TMEM lane quarter) and the tile's
-//               columns in panels of 64.  The residual's panel comes by TMA into the very
-//               buffer that the output panel leaves from (a lane adds and overwrites its
-//               own 16-byte pieces), two panels a warp: while one is computed, the other's
-//               store drains and the next residual panel loads.
+//   warps 2..   epilogue: each warp owns 32 rows (a TMEM lane quarter) x 64 columns.  The
+//               residual's panel comes by TMA into the very buffer that the output panel
+//               leaves from (a lane adds and overwrites its own 16-byte pieces); the next
+//               tile's is asked for as soon as that store has read the buffer.
 //
 // At the widths of graph layers (K and N of a few hundred) the kernel is bound by HBM:
 // A, residual, out and the kept z are each moved once.  A 32-column group of the 8-bit
@@ -36,22 +35,23 @@ namespace {
 constexpr int BM = 128;
 constexpr int BK = 64;
 
+// A warp of the epilogue owns 32 rows x 64 columns of the tile: one panel of output /
+// residual.  The 256-wide tile takes a whole SM (16 epilogue warps);
+// narrower tiles share it (2 and 3 CTAs), so that as many warps work on epilogues.
 template <int BN>
 struct LSmem {
-  static constexpr int kEpi = BN >= 128 ? 8 : 4;             // epilogue warps
-  static constexpr int kCols = BN / (kEpi / 4);              // columns of a warp
-  static constexpr int kPanels = kCols / 64;
+  static constexpr int kEpi = BN / 16;                       // epilogue warps
+  static constexpr int kCtas = BN == 256 ? 1 : (BN == 128 ? 2 : 3);
   static constexpr int kThreads = 64 + 32 * kEpi;
   static constexpr int kABytes = BM * BK * 2;
   static constexpr int kBBytes = BN * BK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kOutBytes = kEpi * 2 * 4096;          // two 32 x 64 bf16 panels a warp
-  static constexpr int kCodeBytes = kEpi * 2048;             // one 32 x 64 code panel a warp
-  static constexpr int kBudget = 226 * 1024 - kOutBytes - kCodeBytes;
-  static constexpr int kStages = kBudget / kStageBytes > 8 ? 8 : kBudget / kStageBytes;
+  static constexpr int kOutBytes = kEpi * 4096;              // a 32 x 64 bf16 panel a warp
+  static constexpr int kBudget = 224 * 1024 / kCtas - 2048 - kOutBytes;
+  static constexpr int kStages = kBudget / kStageBytes > 4 ? 4 : kBudget / kStageBytes;
   static constexpr int kTmemCols = 2 * BN;
-  static constexpr int kBytes = kStages * kStageBytes + kOutBytes + kCodeBytes + 1024 /*align*/;
-  static_assert(kStages >= 3 && kBytes <= 226 * 1024, "linear: shared memory");
+  static constexpr int kBytes = kStages * kStageBytes + kOutBytes + 1024 /*align*/;
+  static_assert(kStages >= 2 && kCtas * (kBytes + 1024) <= 227 * 1024 && kCtas * kTmemCols <= 512, "linear: resources");
 };
 
 // keeps the sign of what a ReLU reads: a positive value's code is at least 1
@@ -67,15 +67,14 @@ __device__ __forceinline__ uint2 codes8_relu(const float* v, float inv) {
 }
 
 template <int BN>
-__global__ void __launch_bounds__(LSmem<BN>::kThreads, 1)
+__global__ void __launch_bounds__(LSmem<BN>::kThreads, LSmem<BN>::kCtas)
     linear_fwd_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
-                      const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmO,
-                      const __grid_constant__ CUtensorMap tmQ, LinearArgs a) {
+                      const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmO, LinearArgs a) {
   GB_PDL_ENTRY();
   using S = LSmem<BN>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2], res_full[S::kEpi][2];
+  __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2], res_full[S::kEpi];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
@@ -87,7 +86,6 @@ __global__ void __launch_bounds__(LSmem<BN>::kThreads, 1)
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* out_area = smem + kStages * S::kStageBytes;
-  uint8_t* code_area = out_area + S::kOutBytes;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
@@ -99,8 +97,8 @@ __global__ void __launch_bounds__(LSmem<BN>::kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], S::kEpi);
-      for (int w = 0; w < S::kEpi; ++w) mbar_init(&res_full[w][b], 1);
     }
+    for (int w = 0; w < S::kEpi; ++w) mbar_init(&res_full[w], 1);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -177,32 +175,26 @@ __global__ void __launch_bounds__(LSmem<BN>::kThreads, 1)
   } else {
     const int w = warp - 2;
     const int quarter = warp & 3;  // TMEM lanes that this warp may read
-    const int col0 = (w / 4) * S::kCols;
-    uint8_t* panel[2] = {out_area + w * 8192, out_area + w * 8192 + 4096};
-    uint8_t* codes = code_area + w * 2048;
+    const int col0 = (w / 4) * 64;
+    uint8_t* panel = out_area + w * 4096;
     const uint64_t key = a.dropout_p > 0.f ? hop_key(static_cast<uint64_t>(a.counters[0]) ^ 0xD80Full,
                                                      static_cast<uint64_t>(a.counters[1]),
                                                      static_cast<uint64_t>(a.counters[2]), a.dropout_salt)
                                            : 0ull;
     const uint32_t thr8 = dropout_thr8(a.dropout_p);
     const float keep_scale = dropout_scale8(thr8);
+    const bool bias16 = (reinterpret_cast<uintptr_t>(a.bias) & 15u) == 0;
     const int n_pad = (a.N + 7) / 8 * 8;
     const int n_code = (a.N + 31) / 32 * 32;
-    uint32_t pc = 0, asked = 0;  // panels done, residual panels asked for
-    auto ask = [&](int64_t t, int p) {  // lane 0: the residual of panel p of tile t into buffer asked & 1
-      const int b = asked & 1;
-      mbar_expect_tx(&res_full[w][b], 4096);
-      tma_load_2d(panel[b], &tmR, &res_full[w][b], static_cast<int>(t % n_tiles) * BN + col0 + p * 64,
+    auto ask = [&](int64_t t) {  // lane 0: tile t's residual panel
+      mbar_expect_tx(&res_full[w], 4096);
+      tma_load_2d(panel, &tmR, &res_full[w], static_cast<int>(t % n_tiles) * BN + col0,
                   static_cast<int>(t / n_tiles) * BM + quarter * 32);
     };
-    if (a.residual) {
-      if (lane == 0) ask(blockIdx.x, 0);
-      asked = 1;
-    }
-    int lt = 0;
-    bool stop = false;
-    for (int64_t t = blockIdx.x; t < tiles && !stop; t += gridDim.x, ++lt) {
-      const int m0 = static_cast<int>(t / n_tiles) * BM + quarter * 32, n0 = static_cast<int>(t % n_tiles) * BN;
+    if (a.residual && lane == 0) ask(blockIdx.x);
+    int lt = 0, taken = 0;  // tiles begun, residual panels that have arrived
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++lt) {
+      const int m0 = static_cast<int>(t / n_tiles) * BM + quarter * 32, nc0 = static_cast<int>(t % n_tiles) * BN + col0;
       const int m = m0 + lane;
       const bool live = m < M;
       const bool slab_full = m0 + 32 <= M;  // rows past M are not written: no TMA store of such a slab
@@ -213,137 +205,132 @@ __global__ void __launch_bounds__(LSmem<BN>::kThreads, 1)
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t trow = tmem_base + static_cast<uint32_t>(ab * BN) + (static_cast<uint32_t>(quarter * 32) << 16);
-#pragma unroll 1
-      for (int p = 0; p < S::kPanels; ++p, ++pc) {
-        const int b = pc & 1;
-        const int nc0 = n0 + col0 + p * 64;
-        if (a.residual) {
-          // the other buffer's store has been read: ask for the next panel into it
-          const bool more = p + 1 < S::kPanels || t + gridDim.x < tiles;
-          if (lane == 0) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            if (more) {
-              if (p + 1 < S::kPanels)
-                ask(t, p + 1);
-              else
-                ask(t + gridDim.x, 0);
-            }
-          }
-          if (more) ++asked;
-          if (!mbar_wait(&res_full[w][b], (pc >> 1) & 1u, &abort_flag)) {
-            if (lane == 0) set_error(a.err, kErrMmaTimeout);
-            abort_flag = 1;
-            stop = true;
-            break;
-          }
-        } else if (lane == 0) {
-          // buffer b left two panels ago, the code panel one panel ago
-          if (a.q8.q)
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          else
-            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      if (a.residual) {
+        if (!mbar_wait(&res_full[w], lt & 1u, &abort_flag)) {
+          if (lane == 0) set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          break;
         }
+        taken = lt + 1;
+      } else {
+        // the last tile's panels have left
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
-        if (nc0 < a.N) {
+      }
+      const uint32_t trow =
+          tmem_base + static_cast<uint32_t>(ab * BN + col0) + (static_cast<uint32_t>(quarter * 32) << 16);
+      if (nc0 < a.N) {
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            const int nc = nc0 + h * 32;
-            float v[32];
-            tmem_ld32(trow + static_cast<uint32_t>(col0 + p * 64 + h * 32), v);
-            if (nc + 32 <= a.N) {
-              if (a.bias) {
+        for (int h = 0; h < 2; ++h) {
+          const int nc = nc0 + h * 32;
+          const bool whole = nc + 32 <= a.N;
+          float v[32];
+          tmem_ld32(trow + h * 32, v);
+          if (whole) {
+            if (a.bias) {
+              if (bias16) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                  const float4 b4 = __ldg(reinterpret_cast<const float4*>(a.bias + nc + j));
+                  v[j] += b4.x, v[j + 1] += b4.y, v[j + 2] += b4.z, v[j + 3] += b4.w;
+                }
+              } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] += __ldg(a.bias + nc + j);
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = nc + j < a.N ? v[j] + (a.bias ? __ldg(a.bias + nc + j) : 0.f) : 0.f;
             }
-            if (a.z && live) {
-              __nv_bfloat16* dst = a.z + static_cast<int64_t>(m) * a.ldz + nc;
+          } else {
 #pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                if (nc + j < n_pad) *reinterpret_cast<uint4*>(dst + j) = f32_to_bf16x8(v + j);
-            }
-            if (a.q8.q && nc < n_code) {
-              uint32_t mx = 0;
-#pragma unroll
-              for (int j = 0; j < 32; j += 8) mx = max(mx, abs_max_bits8(v + j));
-              const uint32_t byte = group8_byte(mx);
-              const float inv = group8_inv(byte);
-              uint2 c[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) c[j] = a.act == kActRelu ? codes8_relu(v + 8 * j, inv) : codes8(v + 8 * j, inv);
-              if (live) a.q8.e[static_cast<int64_t>(m) * a.q8.lde + (nc >> 5)] = static_cast<uint8_t>(byte);
-              uint4* dst;
-              if (slab_full) {
-                // 64-byte rows in the 64B-swizzled layout of the store's map
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  dst = reinterpret_cast<uint4*>(codes + lane * 64 + (((h * 2 + u) ^ ((lane >> 1) & 3)) << 4));
-                  *dst = make_uint4(c[2 * u].x, c[2 * u].y, c[2 * u + 1].x, c[2 * u + 1].y);
-                }
-              } else if (live) {
-                dst = reinterpret_cast<uint4*>(a.q8.q + static_cast<int64_t>(m) * a.q8.ldq + nc);
-                dst[0] = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
-                dst[1] = make_uint4(c[2].x, c[2].y, c[3].x, c[3].y);
-              }
-            }
-            if (a.act == kActRelu) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];  // a NaN stays
-            } else if (a.act == kActGelu) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = gelu(v[j]);
-            } else if (a.act == kActSilu) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = silu(v[j]);
-            }
-            if (a.dropout_p > 0.f) {
-              const uint64_t base = static_cast<uint64_t>(m) * static_cast<uint64_t>(a.ldo) + static_cast<uint64_t>(nc);
-              const uint32_t keep = dropout_keep_bits(key, base, 32, thr8);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = (keep >> j) & 1u ? v[j] * keep_scale : 0.f;
-            }
-            uint8_t* prow = panel[b] + lane * 128;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4* piece = reinterpret_cast<uint4*>(prow + (((h * 4 + q) ^ (lane & 7)) << 4));
-              if (a.residual) {
-                float r[8];
-                bf16x8_to_f32(*piece, r);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[8 * q + j] = nc + 8 * q + j < a.N ? v[8 * q + j] + r[j] : 0.f;
-              }
-              if (slab_full)
-                *piece = f32_to_bf16x8(v + 8 * q);
-              else if (live && nc + 8 * q < n_pad)
-                *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(m) * a.ldo + nc + 8 * q) = f32_to_bf16x8(v + 8 * q);
-            }
+            for (int j = 0; j < 32; ++j) v[j] = nc + j < a.N ? v[j] + (a.bias ? __ldg(a.bias + nc + j) : 0.f) : 0.f;
           }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          if (slab_full && nc0 < a.N) {
-            tma_store_2d(&tmO, panel[b], nc0, m0);
-            if (a.q8.q) tma_store_2d(&tmQ, codes, nc0, m0);
+          if (a.z && live) {
+            __nv_bfloat16* dst = a.z + static_cast<int64_t>(m) * a.ldz + nc;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (nc + j < n_pad) *reinterpret_cast<uint4*>(dst + j) = f32_to_bf16x8(v + j);
           }
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          if (a.q8.q && nc < n_code) {
+            const float top = max_nan(abs_max3(abs_max8(v), abs_max8(v + 8), abs_max8(v + 16)), abs_max8(v + 24));
+            const uint32_t byte = group8_byte(top);
+            const float inv = group8_inv(byte);
+            if (live) a.q8.e[static_cast<int64_t>(m) * a.q8.lde + (nc >> 5)] = static_cast<uint8_t>(byte);
+            uint32_t c[8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const uint2 cu = a.act == kActRelu ? codes8_relu(v + 8 * u, inv) : codes8(v + 8 * u, inv);
+              c[2 * u] = cu.x, c[2 * u + 1] = cu.y;
+            }
+            // neighbouring lanes trade halves, so that a store writes whole 32-byte sectors:
+            // first the even lane's row (16 bytes by each), then the odd lane's
+            const bool odd = lane & 1;
+            uint4 first, second;
+            {
+              uint32_t got[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) got[u] = __shfl_xor_sync(0xffffffffu, odd ? c[u] : c[4 + u], 1);
+              first = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(c[0], c[1], c[2], c[3]);
+              second = odd ? make_uint4(c[4], c[5], c[6], c[7]) : make_uint4(got[0], got[1], got[2], got[3]);
+            }
+            const int me = m - (lane & 1);
+            int8_t* dst = a.q8.q + static_cast<int64_t>(me) * a.q8.ldq + nc + (odd ? 16 : 0);
+            if (me < M) *reinterpret_cast<uint4*>(dst) = first;
+            if (me + 1 < M) *reinterpret_cast<uint4*>(dst + a.q8.ldq) = second;
+          }
+          if (a.act == kActRelu) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];  // a NaN stays
+          } else if (a.act == kActGelu) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) gelu2(v + j);
+          } else if (a.act == kActSilu) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) silu2(v + j);
+          }
+          if (a.dropout_p > 0.f) {
+            const uint64_t base = static_cast<uint64_t>(m) * static_cast<uint64_t>(a.ldo) + static_cast<uint64_t>(nc);
+            const uint32_t keep = dropout_keep_bits(key, base, 32, thr8);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = (keep >> j) & 1u ? v[j] * keep_scale : 0.f;
+          }
+          uint8_t* prow = panel + lane * 128;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4* piece = reinterpret_cast<uint4*>(prow + (((h * 4 + q) ^ (lane & 7)) << 4));
+            if (a.residual) {
+              float r[8];
+              bf16x8_to_f32(*piece, r);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[8 * q + j] += r[j];
+              if (!whole) mask8(v + 8 * q, (nc >> 3) + q, a.N);
+            }
+            if (slab_full)
+              *piece = f32_to_bf16x8(v + 8 * q);
+            else if (live && nc + 8 * q < n_pad)
+              *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(m) * a.ldo + nc + 8 * q) = f32_to_bf16x8(v + 8 * q);
+          }
         }
       }
+      // the accumulator is read: the products of the tile after the next may start
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[ab]);
+      if (lane == 0) {
+        mbar_arrive(&acc_empty[ab]);
+        if (slab_full && nc0 < a.N) tma_store_2d(&tmO, panel, nc0, m0);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        if (a.residual && t + gridDim.x < tiles) {
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          ask(t + gridDim.x);
+        }
+      }
     }
     if (lane == 0) {
       // the panels are in shared memory that ends with the CTA: wait for the stores'
       // reads, and after an abort (bounded) for a residual panel still on its way
       asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      for (uint32_t i = pc; i < asked; ++i) {
+      if (abort_flag && a.residual) {
         const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&res_full[w][i & 1], (i >> 1) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
+        while (!mbar_try_wait(&res_full[w], taken & 1u) && globaltimer_ns() - t0 < kWaitNs) {
         }
       }
     }
@@ -363,13 +350,11 @@ void launch_t(const LinearArgs& a, cudaStream_t stream) {
   const CUtensorMap mw = tensor_map_bf16(a.W, a.N, a.K, a.ldw, BN);
   const CUtensorMap mo = tensor_map_bf16(a.out, a.out_rows, n_pad, a.ldo, 32);
   const CUtensorMap mr = a.residual ? tensor_map_bf16(a.residual, a.r_rows, n_pad, a.ldr, 32) : mo;
-  const CUtensorMap mq =
-      a.q8.q ? tensor_map_u8(a.q8.q, a.q_rows, ceil_div(a.N, 32) * 32, a.q8.ldq, 64, 32, CU_TENSOR_MAP_SWIZZLE_64B) : mo;
   auto kern = linear_fwd_kernel<BN>;
   set_smem(reinterpret_cast<const void*>(kern), S::kBytes);
   const int64_t tiles = ceil_div(a.cap, BM) * ceil_div(a.N, BN);
-  launch_k(kern, dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sm_count()))), dim3(S::kThreads), S::kBytes,
-           stream, ma, mw, mr, mo, mq, a);
+  launch_k(kern, dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sm_count() * S::kCtas))), dim3(S::kThreads), S::kBytes,
+           stream, ma, mw, mr, mo, a);
   GB_LAUNCH_CHECK();
 }
 

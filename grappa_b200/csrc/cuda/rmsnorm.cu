@@ -8,9 +8,10 @@
 //
 // Each row is read once and each output written once; a dozen operations an element, so
 // HBM bounds both.  A team of lanes holds a row in registers, eight columns (one or two
-// 16-byte loads) a lane and step: 4 to 32 lanes for rows of up to 32 * 8 columns, a warp
-// with up to four steps for up to 1024, a whole CTA above.  The row sums are shuffles (one
-// shared-memory exchange for CTA teams).  All sums and statistics are fp32.
+// 16-byte loads) a lane, two rows at a time: 4 to 32 lanes for rows of up to 256 columns, two
+// to eight warps up to 2048, a whole CTA with two or four steps above.  The row sums are
+// shuffles, and one shared-memory exchange for teams of several warps.  All sums and
+// statistics are fp32.
 //
 // dgamma: a lane sums its columns over the rows of its team, the CTA joins its teams in
 // shared memory in a fixed order and writes one part, and a second kernel sums the parts
@@ -28,43 +29,56 @@ namespace {
 constexpr int kThreads = 256;
 
 // Eight columns of a row as they lie in memory, so that every load of a step is issued
-// before the first conversion: kind 0 bf16, 1 fp32, 2 codes.
+// before the first conversion.  Kinds: bf16, fp32, codes.
+enum Kind : int { kBf = 0, kF32 = 1, kQ8 = 2 };
+template <int K>
 struct Raw8 {
-  uint4 a, b;
+  uint32_t w[K == kF32 ? 8 : (K == kBf ? 4 : 2)];
 };
-__device__ __forceinline__ Raw8 raw_load(const void* base, int64_t at, int kind) {
-  Raw8 r;
-  if (kind == 2) {
+template <int K>
+__device__ __forceinline__ Raw8<K> raw_zero() {
+  Raw8<K> r;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(r.w) / 4); ++i) r.w[i] = 0u;
+  return r;
+}
+template <int K>
+__device__ __forceinline__ Raw8<K> raw_load(const void* base, int64_t at) {
+  Raw8<K> r;
+  if constexpr (K == kQ8) {
     const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(base) + at);
-    r.a = make_uint4(q.x, q.y, 0u, 0u);
-  } else if (kind == 1) {
+    r.w[0] = q.x, r.w[1] = q.y;
+  } else if constexpr (K == kF32) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + at);
-    r.a = p[0];
-    r.b = p[1];
+    const uint4 a = p[0], b = p[1];
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+    r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
   } else {
-    r.a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at);
+    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at);
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
   }
   return r;
 }
-__device__ __forceinline__ void raw_values(const Raw8& r, int kind, float scale, float* v) {
-  if (kind == 2) {
-    values8(make_uint2(r.a.x, r.a.y), scale, v);
-  } else if (kind == 1) {
-    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+template <int K>
+__device__ __forceinline__ void raw_values(const Raw8<K>& r, float scale, float* v) {
+  if constexpr (K == kQ8) {
+    values8(make_uint2(r.w[0], r.w[1]), scale, v);
+  } else if constexpr (K == kF32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i]);
   } else {
-    bf16x8_to_f32(r.a, v);
+    bf16x8_to_f32(make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]), v);
   }
 }
-__device__ __forceinline__ void store_any(void* base, int64_t at, bool f32, const float* v) {
-  if (f32)
+template <int K>
+__device__ __forceinline__ void store_kind(void* base, int64_t at, const float* v) {
+  if constexpr (K == kF32)
     store8(static_cast<float*>(base) + at, v);
   else
     store8(static_cast<__nv_bfloat16*>(base) + at, v);
 }
 
-// sum over the team of R values a lane; CTA teams exchange through sh[R][8]
+// sum over the team of R values a lane; teams of several warps exchange through sh[R][8]
 template <int TEAM, int R>
 __device__ __forceinline__ void team_sum(float (&s)[R], float (*sh)[8]) {
 #pragma unroll
@@ -73,7 +87,8 @@ __device__ __forceinline__ void team_sum(float (&s)[R], float (*sh)[8]) {
     for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
   }
   if constexpr (TEAM > 32) {
-    const int w = threadIdx.x >> 5;
+    constexpr int kWarps = TEAM / 32;
+    const int w = threadIdx.x >> 5, w0 = w / kWarps * kWarps;
     __syncthreads();  // the last exchange has been read
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
@@ -84,26 +99,30 @@ __device__ __forceinline__ void team_sum(float (&s)[R], float (*sh)[8]) {
     for (int r = 0; r < R; ++r) {
       s[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[r] += sh[r][i];
+      for (int i = 0; i < kWarps; ++i) s[r] += sh[r][w0 + i];
     }
   }
 }
 
-template <int TEAM, int NV, int R>
-__global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
+template <int K, int TEAM, int NV, int R>
+__global__ void __launch_bounds__(kThreads, NV * R <= 2 ? 4 : 2) rmsnorm_fwd_kernel(RmsNormArgs a) {
   GB_PDL_ENTRY();
   __shared__ float sh[R][8];
   constexpr int kTeams = kThreads / TEAM;
   const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
   const int n = live_rows(a.n_ptr, a.cap);
-  const int kind = a.f32 ? 1 : 0;
   const int chunks = (a.dim + 7) / 8;
   const int qchunks = a.q8.q ? (a.dim + 31) / 32 * 4 : chunks;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
+  float gam[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) gam[i][j] = (i * TEAM + t) * 8 + j < a.dim ? __ldg(a.gamma + (i * TEAM + t) * 8 + j) : 0.f;
   // a CTA takes kTeams * R consecutive rows at a time (uniform trip count per warp)
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * R; base < n;
        base += static_cast<int64_t>(gridDim.x) * kTeams * R) {
-    Raw8 raw[R][NV], rr[R][NV];
+    Raw8<K> raw[R][NV], rr[R][NV];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = base + r * kTeams + team;
@@ -111,9 +130,8 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
       for (int i = 0; i < NV; ++i) {
         const int c = i * TEAM + t;
         const bool on = row < n && c < chunks;
-        raw[r][i].a = raw[r][i].b = rr[r][i].a = rr[r][i].b = make_uint4(0u, 0u, 0u, 0u);
-        if (on) raw[r][i] = raw_load(a.x, row * a.ldx + c * 8, kind);
-        if (on && a.residual) rr[r][i] = raw_load(a.residual, row * a.ldr + c * 8, kind);
+        raw[r][i] = on ? raw_load<K>(a.x, row * a.ldx + c * 8) : raw_zero<K>();
+        rr[r][i] = on && a.residual ? raw_load<K>(a.residual, row * a.ldr + c * 8) : raw_zero<K>();
       }
     }
     float v[R][NV][8], ss[R];
@@ -124,18 +142,16 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = i * TEAM + t;
-        raw_values(raw[r][i], kind, 0.f, v[r][i]);
+        raw_values<K>(raw[r][i], 0.f, v[r][i]);
         if (a.residual) {
           float w[8];
-          raw_values(rr[r][i], kind, 0.f, w);
+          raw_values<K>(rr[r][i], 0.f, w);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[r][i][j] += w[j];
-            if (!a.f32) v[r][i][j] = __bfloat162float(__float2bfloat16_rn(v[r][i][j]));
-          }
+          for (int j = 0; j < 8; ++j) v[r][i][j] += w[j];
+          if constexpr (K == kBf) bf16x8_to_f32(f32_to_bf16x8(v[r][i]), v[r][i]);
         }
         mask8(v[r][i], c, a.dim);
-        if (a.s_out && row < n && c < chunks) store_any(a.s_out, row * a.lds + c * 8, a.f32, v[r][i]);
+        if (a.s_out && row < n && c < chunks) store_kind<K>(a.s_out, row * a.lds + c * 8, v[r][i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss[r] = fmaf(v[r][i][j] * inv_dim, v[r][i][j], ss[r]);
       }
@@ -144,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = base + r * kTeams + team;
-      const float rs = 1.f / sqrtf(ss[r] + a.eps);
+      const float rs = rsqrtf(ss[r] + a.eps);
       if (t == 0 && row < n) a.rstd[row] = rs;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -153,13 +169,16 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           v[r][i][j] *= rs;
-          y[j] = c * 8 + j < a.dim ? v[r][i][j] * __ldg(a.gamma + c * 8 + j) : 0.f;
+          y[j] = v[r][i][j] * gam[i][j];
         }
-        if (row < n && c < chunks) store8(a.y + row * a.ldy + c * 8, y);
+        if (row < n && c < chunks) {
+          mask8(y, c, a.dim);  // an infinite or NaN row: its pad columns stay zero
+          store8(a.y + row * a.ldy + c * 8, y);
+        }
         if (a.q8.q) {
-          uint32_t m = abs_max_bits8(v[r][i]);
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          float m = abs_max8(v[r][i]);
+          m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
           const uint32_t byte = group8_byte(m);
           if (row < n && c < qchunks) {
             *reinterpret_cast<uint2*>(a.q8.q + row * a.q8.ldq + c * 8) = codes8(v[r][i], group8_inv(byte));
@@ -171,8 +190,9 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_fwd_kernel(RmsNormArgs a) {
   }
 }
 
-template <int TEAM, int NV, int R>
-__global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a) {
+template <int KY, int KX, int KD, int TEAM, int NV, int R>
+__global__ void __launch_bounds__(kThreads, NV > 1 ? 1 : (KY == kF32 || KX == kF32 || KD == kF32 ? 2 : 3))
+    rmsnorm_bwd_kernel(RmsNormBwdArgs a) {
   GB_PDL_ENTRY();
   __shared__ float sh[R][8];
   extern __shared__ float parts[];  // [kTeams][TEAM * NV * 8]
@@ -181,7 +201,6 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a)
   const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
   const int n = live_rows(a.n_ptr, a.cap);
   const int n_res = a.dres ? min(live_rows(a.n_res_ptr, a.res_cap), n) : 0;
-  const int ydk = a.dy_f32 ? 1 : 0, xk = a.x ? (a.x_f32 ? 1 : 0) : 2, rk = a.dres_f32 ? 1 : 0;
   const int chunks = (a.dim + 7) / 8;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
   float acc[NV][8], gam[NV][8];
@@ -196,7 +215,9 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a)
   }
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * R; base < n;
        base += static_cast<int64_t>(gridDim.x) * kTeams * R) {
-    Raw8 yr[R][NV], xr[R][NV], rr[R][NV];
+    Raw8<KY> yr[R][NV];
+    Raw8<KX> xr[R][NV];
+    Raw8<KD> rr[R][NV];
     uint32_t eb[R][NV];
     float rs[R];
 #pragma unroll
@@ -206,18 +227,16 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = i * TEAM + t;
-        yr[r][i].a = yr[r][i].b = xr[r][i].a = xr[r][i].b = rr[r][i].a = rr[r][i].b = make_uint4(0u, 0u, 0u, 0u);
-        eb[r][i] = 0;
-        if (row < n && c < chunks) {
-          yr[r][i] = raw_load(a.dy, row * a.lddy + c * 8, ydk);
-          if (xk == 2) {
-            xr[r][i] = raw_load(a.q8.q, row * a.q8.ldq + c * 8, 2);
-            eb[r][i] = a.q8.e[row * a.q8.lde + (c >> 2)];
-          } else {
-            xr[r][i] = raw_load(a.x, row * a.ldx + c * 8, xk);
-          }
-          if (row < n_res) rr[r][i] = raw_load(a.dres, row * a.lddr + c * 8, rk);
+        const bool on = row < n && c < chunks;
+        yr[r][i] = on ? raw_load<KY>(a.dy, row * a.lddy + c * 8) : raw_zero<KY>();
+        if constexpr (KX == kQ8) {
+          xr[r][i] = on ? raw_load<KX>(a.q8.q, row * a.q8.ldq + c * 8) : raw_zero<KX>();
+          eb[r][i] = on ? a.q8.e[row * a.q8.lde + (c >> 2)] : 0u;
+        } else {
+          xr[r][i] = on ? raw_load<KX>(a.x, row * a.ldx + c * 8) : raw_zero<KX>();
+          eb[r][i] = 0u;
         }
+        rr[r][i] = on && row < n_res ? raw_load<KD>(a.dres, row * a.lddr + c * 8) : raw_zero<KD>();
       }
     }
     float dy[R][NV][8], xh[R][NV][8], dot[R];
@@ -227,13 +246,13 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = i * TEAM + t;
-        raw_values(yr[r][i], ydk, 0.f, dy[r][i]);
-        raw_values(xr[r][i], xk, group8_scale(eb[r][i]), xh[r][i]);
+        raw_values<KY>(yr[r][i], 0.f, dy[r][i]);
+        raw_values<KX>(xr[r][i], group8_scale(eb[r][i]), xh[r][i]);
         mask8(dy[r][i], c, a.dim);
         mask8(xh[r][i], c, a.dim);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (xk != 2) xh[r][i][j] *= rs[r];
+          if constexpr (KX != kQ8) xh[r][i][j] *= rs[r];
           const float p = dy[r][i][j] * xh[r][i][j];
           acc[i][j] += p;
           dot[r] = fmaf(p, gam[i][j], dot[r]);
@@ -250,16 +269,16 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(RmsNormBwdArgs a)
         const int c = i * TEAM + t;
         if (row < n && c < chunks) {
           float dr[8], o[8];
-          raw_values(rr[r][i], rk, 0.f, dr);
-          mask8(dr, c, a.dim);
+          raw_values<KD>(rr[r][i], 0.f, dr);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             o[j] = fmaf(rs[r], fmaf(-xh[r][i][j], mean, gam[i][j] * dy[r][i][j]), dr[j]);
+          mask8(o, c, a.dim);
           if (a.clear_dy) {
             const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            store_any(a.dy, row * a.lddy + c * 8, a.dy_f32, z);
+            store_kind<KY>(a.dy, row * a.lddy + c * 8, z);
           }
-          store_any(a.dx, row * a.lddx + c * 8, a.dx_f32, o);
+          store_kind<KD>(a.dx, row * a.lddx + c * 8, o);
         }
       }
     }
@@ -309,30 +328,62 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// rows a CTA takes at a time, and the CTAs for cap rows: all of them at once up to
-// kCtasPerSm on every SM
-constexpr int kCtasPerSm = 4;
+// CTAs for cap rows: one pass of rows each, up to as many as the SMs hold at once
+constexpr int kBwdCtasPerSm = 3;
 template <int TEAM, int R>
-int grid_rows(int cap, int num_sms) {
-  return static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(ceil_div(cap, kThreads / TEAM * R), static_cast<int64_t>(num_sms) * kCtasPerSm)));
-}
+int64_t passes(int cap) { return std::max<int64_t>(1, ceil_div(cap, kThreads / TEAM * R)); }
 
-template <int TEAM, int NV, int R>
-void fwd_t(const RmsNormArgs& a, cudaStream_t stream) {
-  // not persistent: one pass of rows a CTA, the hardware refills the SMs
-  const int64_t grid = ceil_div(a.cap, kThreads / TEAM * R);
-  launch_k(rmsnorm_fwd_kernel<TEAM, NV, R>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+template <int K, int TEAM, int NV, int R>
+void fwd_t(const RmsNormArgs& a, int num_sms, cudaStream_t stream) {
+  const int64_t grid = std::min<int64_t>(passes<TEAM, R>(a.cap), static_cast<int64_t>(num_sms) * 4);
+  launch_k(rmsnorm_fwd_kernel<K, TEAM, NV, R>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
   GB_LAUNCH_CHECK();
 }
 
-template <int TEAM, int NV, int R>
+template <int K>
+void fwd_k(const RmsNormArgs& a, int num_sms, cudaStream_t stream) {
+  const int d = a.dim;
+  if (d <= 32) return fwd_t<K, 4, 1, 2>(a, num_sms, stream);
+  if (d <= 64) return fwd_t<K, 8, 1, 2>(a, num_sms, stream);
+  if (d <= 128) return fwd_t<K, 16, 1, 2>(a, num_sms, stream);
+  if (d <= 256) return fwd_t<K, 32, 1, 2>(a, num_sms, stream);
+  if (d <= 512) return fwd_t<K, 64, 1, 2>(a, num_sms, stream);
+  if (d <= 1024) return fwd_t<K, 128, 1, 2>(a, num_sms, stream);
+  if (d <= 2048) return fwd_t<K, 256, 1, 2>(a, num_sms, stream);
+  if (d <= 4096) return fwd_t<K, 256, 2, 1>(a, num_sms, stream);
+  return fwd_t<K, 256, 4, 1>(a, num_sms, stream);
+}
+
+template <int KY, int KX, int KD, int TEAM, int NV, int R>
 void bwd_t(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
-  const int grid = grid_rows<TEAM, R>(a.cap, num_sms);
+  const int grid = static_cast<int>(std::min<int64_t>(passes<TEAM, R>(a.cap), static_cast<int64_t>(num_sms) * kBwdCtasPerSm));
   const size_t smem = TEAM < kThreads ? sizeof(float) * kThreads * NV * 8 : 0;
-  launch_k(rmsnorm_bwd_kernel<TEAM, NV, R>, dim3(grid), dim3(kThreads), smem, stream, a);
+  launch_k(rmsnorm_bwd_kernel<KY, KX, KD, TEAM, NV, R>, dim3(grid), dim3(kThreads), smem, stream, a);
   GB_LAUNCH_CHECK();
   launch_sum_parts(a.work, grid, a.dim, a.dim, a.dgamma, a.accumulate, stream);
+}
+
+template <int KY, int KX, int KD>
+void bwd_k(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
+  const int d = a.dim;
+  if (d <= 64) return bwd_t<KY, KX, KD, 8, 1, 2>(a, num_sms, stream);
+  if (d <= 128) return bwd_t<KY, KX, KD, 16, 1, 2>(a, num_sms, stream);
+  if (d <= 256) return bwd_t<KY, KX, KD, 32, 1, 2>(a, num_sms, stream);
+  if (d <= 512) return bwd_t<KY, KX, KD, 64, 1, 2>(a, num_sms, stream);
+  if (d <= 1024) return bwd_t<KY, KX, KD, 128, 1, 2>(a, num_sms, stream);
+  if (d <= 2048) return bwd_t<KY, KX, KD, 256, 1, 2>(a, num_sms, stream);
+  if (d <= 4096) return bwd_t<KY, KX, KD, 256, 2, 1>(a, num_sms, stream);
+  return bwd_t<KY, KX, KD, 256, 4, 1>(a, num_sms, stream);
+}
+
+template <int KY, int KX>
+void bwd_yx(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
+  a.dx_f32 ? bwd_k<KY, KX, kF32>(a, num_sms, stream) : bwd_k<KY, KX, kBf>(a, num_sms, stream);
+}
+template <int KY>
+void bwd_y(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
+  if (!a.x) return bwd_yx<KY, kQ8>(a, num_sms, stream);
+  a.x_f32 ? bwd_yx<KY, kF32>(a, num_sms, stream) : bwd_yx<KY, kBf>(a, num_sms, stream);
 }
 
 }  // namespace
@@ -345,34 +396,16 @@ void launch_sum_parts(const float* part, int parts, int64_t ld, int cols, float*
 }
 
 int64_t rmsnorm_bwd_work_floats(int dim, int cap, int num_sms) {
-  return static_cast<int64_t>(dim) * std::min<int64_t>(std::max(cap, 1), static_cast<int64_t>(num_sms) * kCtasPerSm);
+  return static_cast<int64_t>(dim) * std::min<int64_t>(std::max(cap, 1), static_cast<int64_t>(num_sms) * kBwdCtasPerSm);
 }
 
-void launch_rmsnorm_fwd(const RmsNormArgs& a, cudaStream_t stream) {
+void launch_rmsnorm_fwd(const RmsNormArgs& a, int num_sms, cudaStream_t stream) {
   if (a.cap <= 0) return;
-  const int d = a.dim;
-  if (d <= 32) return fwd_t<4, 1, 2>(a, stream);
-  if (d <= 64) return fwd_t<8, 1, 2>(a, stream);
-  if (d <= 128) return fwd_t<16, 1, 2>(a, stream);
-  if (d <= 256) return fwd_t<32, 1, 2>(a, stream);
-  if (d <= 512) return fwd_t<32, 2, 1>(a, stream);
-  if (d <= 1024) return fwd_t<32, 4, 1>(a, stream);
-  if (d <= 2048) return fwd_t<256, 1, 2>(a, stream);
-  if (d <= 4096) return fwd_t<256, 2, 1>(a, stream);
-  return fwd_t<256, 4, 1>(a, stream);
+  a.f32 ? fwd_k<kF32>(a, num_sms, stream) : fwd_k<kBf>(a, num_sms, stream);
 }
 
 void launch_rmsnorm_bwd(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
-  const int d = a.dim;
-  if (d <= 32) return bwd_t<4, 1, 2>(a, num_sms, stream);
-  if (d <= 64) return bwd_t<8, 1, 2>(a, num_sms, stream);
-  if (d <= 128) return bwd_t<16, 1, 2>(a, num_sms, stream);
-  if (d <= 256) return bwd_t<32, 1, 2>(a, num_sms, stream);
-  if (d <= 512) return bwd_t<32, 2, 1>(a, num_sms, stream);
-  if (d <= 1024) return bwd_t<32, 4, 1>(a, num_sms, stream);
-  if (d <= 2048) return bwd_t<256, 1, 2>(a, num_sms, stream);
-  if (d <= 4096) return bwd_t<256, 2, 1>(a, num_sms, stream);
-  return bwd_t<256, 4, 1>(a, num_sms, stream);
+  a.dy_f32 ? bwd_y<kF32>(a, num_sms, stream) : bwd_y<kBf>(a, num_sms, stream);
 }
 
 }  // namespace dev

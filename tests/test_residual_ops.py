@@ -82,6 +82,7 @@ CASES = [
     ("rmsnorm_bwd", bwd_args, dict(q=Q, q_exp=E), "one of them"),
     ("rmsnorm_bwd", bwd_args, dict(n_res_dev=torch.zeros(1, dtype=torch.int32)), "dres"),
     ("rmsnorm_bwd", bwd_args, dict(dres=z(3, 104)), "rows"),
+    ("rmsnorm_bwd", bwd_args, dict(dres=z(4, 104, F32)), "dtype"),
     ("rmsnorm_bwd", bwd_args, dict(dgamma=torch.zeros(99)), "dgamma"),
     ("rmsnorm_bwd", bwd_args, dict(dy=BUF[:, :104], dx=BUF[:, :104], clear_dy=True), "overlaps"),
     ("rmsnorm_bwd", bwd_args, dict(x=BUF[:, :104], dx=BUF[:, :104]), "overlaps"),
