@@ -12,7 +12,8 @@ One training step of a block GNN, entirely on the device:
 
 Layer programs (kernels in grappa_b200/csrc/cuda):
   SAGE     aggregate [h_dst | mean h_src] -> tcgen05 GEMM (+bias, ReLU, dropout; or the
-           fused softmax cross-entropy of the last layer)
+           fused softmax cross-entropy of the last layer); with norm / residual / GELU / SiLU
+           or activations in 8 bits: RMS norm -> aggregate -> linear with its epilogue
   GCN      in <= out: aggregate (sym. norm) -> GEMM;  in > out: GEMM over the source
            rows -> aggregate with the bias/ReLU/dropout epilogue (DGL's order)
   GIN      aggregate (sum + self) -> GEMM -> BatchNorm+ReLU -> GEMM -> BatchNorm+ReLU
@@ -31,9 +32,11 @@ import math
 import os
 
 import torch
+import torch.nn.functional as F
 
 from grappa_b200 import _native
 from grappa_b200.models.flat import pad8
+from grappa_b200.ops import ref
 from grappa_b200.sampler_gpu import C_EPOCH, C_STEP, GpuNeighborSampler, new_counters
 
 GEMM_STORE_BF16, GEMM_STORE_F32, GEMM_ATOMIC_F32, GEMM_CROSS_ENTROPY = 0, 1, 2, 3
@@ -954,6 +957,173 @@ class SageEngine(BlockEngine):
                    prev["rows"])
 
 
+#: activation functions of the linear kernel's epilogue
+LINEAR_ACTS = {F.relu: 1, ref.gelu: 2, F.silu: 3}
+
+
+def needs_residual_engine(model):
+    """Whether a GraphSAGE model uses what only the residual layers' kernels have."""
+    return bool(model.norm is not None or model.residual
+                or (model.activation is not F.relu and model.activation in LINEAR_ACTS))
+
+
+class ResidualSageEngine(SageEngine):
+    """GraphSAGE with RMS norm, residual layers, GELU / SiLU, and activations kept in 8 bits:
+
+        n = rmsnorm(h_l),  X = [n_dst | mean n_src],  h_{l+1} = h_l[dst] + dropout(act(X W^T + b))
+
+    The linear kernel's epilogue applies bias, activation, dropout and residual.  What the
+    backward pass reads is kept per layer: X (weight gradient), z = X W^T + b (activation)
+    and the norm's input.  ``act_bits=16`` keeps them as bf16 rows; ``act_bits=8`` keeps X, z
+    and the normalised rows in 8 bits, and the bf16 rows themselves live in buffers that all
+    layers share: per hidden layer of width d, 4d + groups bytes a row instead of 8d.
+    The gradient of the residual stream is fp32 and passes through the norms' backward."""
+
+    def __init__(self, *args, act_bits=16, **kw):
+        if act_bits not in (8, 16):
+            raise ValueError("act_bits must be 8 or 16")
+        self.act_bits = int(act_bits)
+        super().__init__(*args, **kw)
+
+    def _make_sampler(self, batch_size, n_nodes_cap, dev):
+        return BlockEngine._make_sampler(self, batch_size, n_nodes_cap, dev)
+
+    def _alloc_layers(self):
+        dev, m, eight = self.device, self.model, self.act_bits == 8
+        bf = dict(dtype=torch.bfloat16, device=dev)
+        f32 = dict(dtype=torch.float32, device=dev)
+        if m.activation not in LINEAR_ACTS:
+            raise ValueError("the GPU engine has ReLU, GELU (tanh form) and SiLU")
+        self.act = LINEAR_ACTS[m.activation]
+
+        def codes(rows, dim):
+            w = (dim + 31) // 32 * 32
+            return dict(q=torch.zeros((rows, w), dtype=torch.int8, device=dev),
+                        q_exp=torch.zeros((rows, w // 32), dtype=torch.uint8, device=dev))
+
+        shared = {}
+
+        def scratch(name, rows, cols, dtype):
+            """Rows that only one layer needs at a time: one buffer for all layers."""
+            n = rows * cols
+            if name not in shared or shared[name].numel() < n:
+                shared[name] = torch.zeros(n, dtype=dtype, device=dev)
+            return lambda: shared[name][:n].view(rows, cols)
+
+        lazy = []  # views of the shared buffers, made when their sizes are known
+        for l, layer in enumerate(m.layers):
+            h = self.L - 1 - l
+            ip, op = pad8(layer.in_feats), pad8(layer.out_feats)
+            K, rows, srows = 2 * ip, self.sm.cap_dst[h], self.sm.cap_src[h]
+            last = l == self.L - 1
+            s = dict(h=h, ip=ip, op=op, K=K, rows=rows, srows=srows, last=last, res=m.has_residual(l),
+                     W=self._seg(layer.seg_w, self.wbf), bias=self._seg(layer.seg_b)[0],
+                     gW=self._seg(layer.seg_w, self.grad), gb=self._seg(layer.seg_b, self.grad)[0])
+            lazy.append((s, "dY", scratch(f"dY{l & 1}", rows, op, torch.bfloat16)))
+            if eight:
+                lazy.append((s, "X", scratch("X", rows, K, torch.bfloat16)))
+                s["Xq"] = codes(rows, K)
+            else:
+                s["X"] = torch.zeros((rows, K), **bf)
+            if last:
+                s["ce_fused"] = op <= 64
+                if not s["ce_fused"]:
+                    s["logits"] = torch.zeros((rows, op), **bf)
+            else:
+                # the residual stream: the norm's backward reads it, or its 8-bit form
+                if eight:
+                    lazy.append((s, "H", scratch(f"H{l & 1}", rows, op, torch.bfloat16)))
+                    s["Z"] = codes(rows, op)
+                else:
+                    s["H"] = torch.zeros((rows, op), **bf)
+                    s["Z"] = dict(z=torch.zeros((rows, op), **bf))
+                if m.norm is None:
+                    s["dH"] = torch.zeros((rows, op), **f32)  # summed into: cleared by its reader
+                else:
+                    lazy.append((s, "dH", scratch(f"dH{l & 1}", rows, op, torch.float32)))
+            if l > 0:
+                lazy.append((s, "dX", scratch("dX", rows, K, torch.bfloat16)))
+                if m.norm is not None:
+                    norm = m.norms[l - 1]
+                    s["norm"] = norm
+                    s["gamma"], s["ggamma"] = self._seg(norm.seg)[0], self._seg(norm.seg, self.grad)[0]
+                    s["rstd"] = torch.zeros(srows, **f32)
+                    lazy.append((s, "N", scratch("N", srows, ip, torch.bfloat16)))
+                    s["dN"] = None  # fp32 sums of the aggregation's backward, cleared by the norm's
+                    lazy.append((s, "dN", scratch(f"dN{ip}", srows, ip, torch.float32)))
+                    s["Nq"] = codes(srows, layer.in_feats) if eight else {}
+            self.lay.append(s)
+        for s, name, view in lazy:
+            s[name] = view()
+
+    def _forward(self, training=True):
+        cu, sm = self.cu, self.sm
+        for l, s in enumerate(self.lay):
+            h = s["h"]
+            src, src_map = self._input(l)
+            if "norm" in s:
+                cu.rmsnorm_fwd(src, s["norm"].dim, sm.n_src(h), s["srows"], s["gamma"], s["norm"].eps, s["N"], s["rstd"],
+                               **(s["Nq"] if training else {}))
+                src = s["N"]
+            cu.aggregate(sm.indptr[h], sm.indices[h], self._n_dst(h), 0, sm.cap_dst[h], src, src_map, s["ip"], AGG_MEAN,
+                         None, None, None, s["X"], s["ip"], 0, 0.0, 0, self.err)
+            if training and "Xq" in s:
+                cu.ckpt8_store(s["X"], s["K"], self._n_dst(h), s["rows"], **s["Xq"])
+            if not s["last"]:
+                p = self.p if training else 0.0
+                cu.linear_fwd(s["X"], s["W"], self._n_dst(h), s["rows"], s["H"], self.err, bias=s["bias"], act=self.act,
+                              residual=self.lay[l - 1]["H"] if s["res"] else None, dropout_p=p,
+                              counters=self.counters if p > 0 else None, salt=l, **(s["Z"] if training else {}))
+            elif s["ce_fused"]:
+                labels, mask, n_sel = self._labels_rows()
+                cu.gemm(s["X"], False, s["W"], False, s["rows"], self._n_dst(h), s["op"], s["K"], None, 1,
+                        self._ce_dummy, GEMM_CROSS_ENTROPY, s["bias"], 0, 0.0, None, 0, labels, self.n_classes, s["dY"],
+                        self.fstats[2:3], self.istats[0:1], None, self._n_dst(h), s["gb"] if training else None,
+                        self.err, bn_for(s["op"]))
+            else:
+                self._gemm(s["X"], False, s["W"], False, s["rows"], self._n_dst(h), s["op"], s["K"], None, 1,
+                           s["logits"], GEMM_STORE_BF16, s["bias"])
+                self._ce(s["logits"], self.n_classes, s["dY"], s["gb"] if training else None, h)
+
+    def _dw8(self, s):
+        """The layer's weight gradient from its 8-bit rows, on the auxiliary stream (``_dw``)."""
+        main = torch.cuda.current_stream(self.device)
+        aux = self._aux_stream()
+        aux.wait_stream(main)
+        with torch.cuda.stream(aux):
+            self.cu.ckpt8_dw(s["dY"], n_dev=self._n_dst(s["h"]), cap=s["rows"], gw=s["gW"][:s["op"]], err=self.err,
+                             **s["Xq"])
+        self._aux_used = True
+
+    def _backward_layer(self, l):
+        cu, sm = self.cu, self.sm
+        s = self.lay[l]
+        h = s["h"]
+        n = self._n_dst(h)
+        if not s["last"]:
+            # dY of this parity is read by layer l + 2's weight gradient on the auxiliary stream
+            self._join_aux()
+            cu.linear_act_bwd(s["dH"], self.model.layers[l].out_feats, n, s["rows"], self.act, s["dY"], s["gb"],
+                              clear_dout="norm" not in s and self.model.norm is None, dropout_p=self.p,
+                              counters=self.counters if self.p > 0 else None, salt=l, ld_mask=s["op"], **s["Z"])
+        if "Xq" in s:
+            self._dw8(s)
+        else:
+            self._dw(s["dY"], s["X"], s["op"], s["K"], s["rows"], n, s["gW"])
+        if l == 0:
+            return
+        self._gemm(s["dY"], False, s["W"], True, s["rows"], n, s["K"], s["op"], None, 1, s["dX"], GEMM_STORE_BF16)
+        prev = self.lay[l - 1]
+        into = s["dN"] if "norm" in s else prev["dH"]
+        cu.aggregate_bwd(sm.indptr[h], sm.indices[h], n, 0, sm.cap_dst[h], s["dX"], s["ip"], 0, 0.0, s["ip"], AGG_MEAN,
+                         None, None, None, into, self.err)
+        if "norm" in s:
+            kept = s["Nq"] if s["Nq"] else {}
+            cu.rmsnorm_bwd(s["dN"], None if kept else prev["H"], s["rstd"], s["gamma"], s["norm"].dim, sm.n_src(h),
+                           s["srows"], prev["dH"], s["ggamma"], dres=s["dH"] if s["res"] else None,
+                           n_res_dev=n if s["res"] else None, clear_dy=True, **kept)
+
+
 class GcnEngine(BlockEngine):
     """GCN (GraphConv norm='both'): D_dst^-1/2 A D_src^-1/2 h W + b.  The projection
     runs first when it narrows the rows (in > out), as DGL does."""
@@ -1429,8 +1599,13 @@ class PinSageEngine(BlockEngine):
 ENGINES = {"sage": SageEngine, "gcn": GcnEngine, "gin": GinEngine, "gat": GatEngine, "pinsage": PinSageEngine}
 
 
-def make_engine(model, *args, **kwargs):
-    """The engine class of ``model.name`` (sage, gcn, gin, gat, pinsage)."""
+def make_engine(model, *args, act_bits=16, **kwargs):
+    """The engine class of ``model.name`` (sage, gcn, gin, gat, pinsage).  ``act_bits=8``
+    (sage): what the backward pass reads is kept in 8 bits."""
+    if model.name == "sage" and (act_bits != 16 or needs_residual_engine(model)):
+        return ResidualSageEngine(model, *args, act_bits=act_bits, **kwargs)
+    if act_bits != 16:
+        raise ValueError(f"act_bits={act_bits} is an option of the sage model, not of {model.name}")
     try:
         cls = ENGINES[model.name]
     except KeyError:

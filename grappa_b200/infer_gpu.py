@@ -12,7 +12,8 @@ its running statistics, on buffers sized for the block.
 import torch
 
 from grappa_b200 import _native
-from grappa_b200.engine import AGG_GCN, AGG_MEAN, AGG_SUM, AGG_WEIGHTED, GEMM_STORE_BF16, gemm_bn
+from grappa_b200.engine import (AGG_GCN, AGG_MEAN, AGG_SUM, AGG_WEIGHTED, GEMM_STORE_BF16, LINEAR_ACTS, gemm_bn,
+                                needs_residual_engine)
 from grappa_b200.models.flat import pad8
 
 
@@ -58,11 +59,25 @@ def _input_rows(ctx, h, n_src, ip):
     return x
 
 
-def _sage(ctx, layer, last, ip_, ix, n_dst, n_src, x):
+def _sage(ctx, model, l, last, ip_, ix, n_dst, n_src, x):
     cu = ctx.cu
+    layer = model.layers[l]
     ip, op = pad8(layer.in_feats), pad8(layer.out_feats)
     R = _rows(n_dst)
     X = ctx.zeros(R, 2 * ip)
+    if needs_residual_engine(model):
+        n = x
+        if model.norm is not None and l > 0:
+            n = torch.zeros_like(x)
+            norm = model.norms[l - 1]
+            cu.rmsnorm_fwd(x, norm.dim, ctx.count(n_src), x.shape[0], ctx.seg(norm.seg, False)[0], norm.eps, n,
+                           torch.zeros(x.shape[0], dtype=torch.float32, device=ctx.dev))
+        cu.aggregate(ip_, ix, None, n_dst, R, n, None, ip, AGG_MEAN, None, None, None, X, ip, 0, 0.0, 0, ctx.err)
+        H = ctx.zeros(R, op)
+        cu.linear_fwd(X, ctx.seg(layer.seg_w), ctx.count(n_dst), R, H, ctx.err, bias=ctx.seg(layer.seg_b, False)[0],
+                      act=0 if last else LINEAR_ACTS[model.activation],
+                      residual=x if model.has_residual(l) else None)
+        return H[:n_dst, :layer.out_feats]
     cu.aggregate(ip_, ix, None, n_dst, R, x, None, ip, AGG_MEAN, None, None, None, X, ip, 0, 0.0, 0, ctx.err)
     H = ctx.zeros(R, op)
     ctx.gemm(X, ctx.seg(layer.seg_w), False, R, ctx.count(n_dst), op, 2 * ip, H, ctx.seg(layer.seg_b, False)[0],
@@ -170,7 +185,7 @@ def infer_layer(model, layer_i, block, h):
     layer = model.layers[layer_i]
     name = model.name
     if name == "sage":
-        out = _sage(ctx, layer, last, ip_, ix, n_dst, n_src, _input_rows(ctx, h, n_src, pad8(layer.in_feats)))
+        out = _sage(ctx, model, layer_i, last, ip_, ix, n_dst, n_src, _input_rows(ctx, h, n_src, pad8(layer.in_feats)))
     elif name == "gcn":
         out = _gcn(ctx, layer, last, ip_, ix, n_dst, n_src, _input_rows(ctx, h, n_src, pad8(layer.in_feats)))
     elif name == "gin":

@@ -12,10 +12,13 @@ import torch.nn.functional as F
 from torch import nn
 
 from grappa_b200.models.flat import FlatModule, pad8
-from grappa_b200.models.layers import GATConv, GINConv, GINMLP, GraphConv, SAGEConv, WeightedSAGEConv
+from grappa_b200.models.layers import GATConv, GINConv, GINMLP, GraphConv, RMSNorm, SAGEConv, WeightedSAGEConv
 from grappa_b200.ops import ref
 
-__all__ = ["SAGE", "GCN", "GAT", "GIN", "PinSAGE", "get_model"]
+__all__ = ["SAGE", "GCN", "GAT", "GIN", "PinSAGE", "get_model", "ACTIVATIONS"]
+
+#: activations by name; the GPU engine knows these functions
+ACTIVATIONS = {"relu": F.relu, "gelu": ref.gelu, "silu": F.silu}
 
 
 class _Base(FlatModule):
@@ -38,17 +41,36 @@ class _Base(FlatModule):
 
 
 class SAGE(_Base):
-    """GraphSAGE, mean aggregator (reference experiments/grappa/train/graphsage.py:11-42)."""
+    """GraphSAGE, mean aggregator (reference experiments/grappa/train/graphsage.py:11-42).
 
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=F.relu, dropout=0.5):
+    ``norm="rms"`` normalises the rows that every layer but the first reads (RMS norm with a
+    learned weight), ``residual=True`` (with the norm) adds the un-normalised destination
+    rows to the output of every hidden layer whose widths agree:
+
+        h_{l+1} = h_l[dst] + dropout(act([n | mean n] W^T + b)),   n = rmsnorm(h_l)
+    """
+
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=F.relu, dropout=0.5, norm=None,
+                 residual=False):
         super().__init__()
+        if norm not in (None, "rms"):
+            raise ValueError(f"unknown norm {norm}: None or 'rms'")
+        if residual and norm is None:
+            raise ValueError("residual layers need norm='rms' (the residual stream grows without it)")
         self.name = "sage"
         self.n_layers, self.n_hidden, self.n_classes = n_layers, n_hidden, n_classes
         self.in_feats = in_feats
+        self.norm, self.residual = norm, bool(residual)
         dims = [in_feats] + [n_hidden] * (n_layers - 1) + [n_classes]
-        self.layers = nn.ModuleList(
-            [SAGEConv(self, f"layers.{i}", dims[i], dims[i + 1]) for i in range(n_layers)]
-        )
+        layers, norms = [], []
+        for i in range(n_layers):
+            # a layer's norm lies with its weights: its gradient is one bucket of the all-reduce
+            if norm is not None and i > 0:
+                norms.append(RMSNorm(self, f"layers.{i}.norm", dims[i]))
+            layers.append(SAGEConv(self, f"layers.{i}", dims[i], dims[i + 1]))
+        self.layers = nn.ModuleList(layers)
+        if norm is not None:
+            self.norms = nn.ModuleList(norms)
         self.dropout = nn.Dropout(dropout)
         self.dropout_p = float(dropout)
         self.activation = activation
@@ -57,14 +79,27 @@ class SAGE(_Base):
     def reset_parameters(self):
         for layer in self.layers:
             layer.reset_parameters()
+        for n in getattr(self, "norms", ()):
+            n.reset_parameters()
+
+    def has_residual(self, l):
+        """Whether layer l adds its destination rows to its output."""
+        layer = self.layers[l]
+        return self.residual and 0 < l < self.n_layers - 1 and layer.in_feats == layer.out_feats
+
+    def run_layer(self, l, block, h):
+        """Layer l with its norm, activation, dropout and residual."""
+        n = self.norms[l - 1](h) if self.norm is not None and l > 0 else h
+        z = self.layers[l](block, n)
+        if l == self.n_layers - 1:
+            return z
+        z = self._drop(self.activation(z), l, pad8(self.layers[l].out_feats))
+        return h[: block.num_dst_nodes()] + z if self.has_residual(l) else z
 
     def forward(self, blocks, x):
         h = x
-        for l, (layer, block) in enumerate(zip(self.layers, blocks)):
-            h = layer(block, h)
-            if l != len(self.layers) - 1:
-                h = self.activation(h)
-                h = self._drop(h, l, pad8(layer.out_feats))
+        for l, block in zip(range(self.n_layers), blocks):
+            h = self.run_layer(l, block, h)
         return h
 
 
@@ -212,11 +247,17 @@ class PinSAGE(_Base):
         return h
 
 
-def get_model(name, n_feat_dim, n_class, num_hidden=128, num_layers=3, dropout=0.5, n_heads=4):
+def get_model(name, n_feat_dim, n_class, num_hidden=128, num_layers=3, dropout=0.5, n_heads=4, activation="relu",
+              norm=None, residual=False):
     """Model factory with the reference's argument mapping
-    (experiments/grappa/train/t10n_train.py:52-101)."""
+    (experiments/grappa/train/t10n_train.py:52-101).  ``activation`` (a name of
+    ``ACTIVATIONS``), ``norm`` and ``residual`` are GraphSAGE's."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation}: one of {', '.join(ACTIVATIONS)}")
     if name == "sage":
-        return SAGE(n_feat_dim, num_hidden, n_class, num_layers, F.relu, dropout)
+        return SAGE(n_feat_dim, num_hidden, n_class, num_layers, ACTIVATIONS[activation], dropout, norm, residual)
+    if activation != "relu" or norm is not None or residual:
+        raise ValueError(f"activation, norm and residual are options of the sage model, not of {name}")
     if name == "gat":
         return GAT(n_feat_dim, num_hidden, n_class, n_heads, num_layers, F.relu, dropout)
     if name == "gcn":

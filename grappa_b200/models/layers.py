@@ -35,6 +35,27 @@ def _cpu_only(x):
         )
 
 
+class RMSNorm(nn.Module):
+    """y = x / sqrt(mean(x^2) + eps) * weight over the feature columns.
+
+    Flat layout: segment [1, pad8(dim)]."""
+
+    def __init__(self, owner, name, dim, eps=1e-5):
+        super().__init__()
+        self.dim, self.eps = int(dim), float(eps)
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.seg = name
+        owner.add_segment(name, 1, dim)
+        owner.bind(self, "weight", name, 0, slice(0, dim))
+
+    def reset_parameters(self):
+        self.weight.fill_(1.0)
+
+    def forward(self, x):
+        _cpu_only(x)
+        return ref.rms_norm(x, self.weight, self.eps)
+
+
 class SAGEConv(nn.Module):
     """out = fc_self(h_dst) + fc_neigh(mean_{u in N(v)} h_u) + bias.
 

@@ -64,3 +64,13 @@ def edge_softmax(block, e):
     ex = torch.exp(e - emax[v])
     den = torch.zeros((n_dst, H), dtype=e.dtype, device=e.device).index_add_(0, v, ex)
     return ex / den[v]
+
+
+def rms_norm(x, weight, eps):
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension."""
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weight
+
+
+def gelu(x):
+    """GELU in its tanh form (the form of the linear kernel's epilogue)."""
+    return torch.nn.functional.gelu(x, approximate="tanh")

@@ -27,7 +27,7 @@ from grappa_b200.dataset.meta import name_to_meta
 from grappa_b200.grad import coverage_all_reduce
 from grappa_b200.models import get_model
 from grappa_b200.train import resilience
-from grappa_b200.train.t10n_train import build_parser, rank_print, save_to_ckpt, set_metrics_sink
+from grappa_b200.train.t10n_train import build_parser, model_options, rank_print, save_to_ckpt, set_metrics_sink
 
 
 def _cpu_full_block(loader):
@@ -64,7 +64,7 @@ def run_cpu(args):
     meta = name_to_meta(args.graph_name)
     torch.manual_seed(args.seed)
     model = get_model(args.model, meta.n_dim, meta.n_label, num_hidden=args.num_hidden, num_layers=args.num_layers,
-                      dropout=args.dropout)
+                      dropout=args.dropout, **model_options(args))
     opt = torch.optim.Adam(model.parameters(), lr=args.lr)
     loader = IsolatedDataloader(torch.device("cpu"), args)
     rank, world = loader.get_rank(), loader.world
@@ -116,11 +116,11 @@ def run_gpu(args):
     meta = name_to_meta(args.graph_name)
     torch.manual_seed(args.seed)
     model = get_model(args.model, meta.n_dim, meta.n_label, num_hidden=args.num_hidden, num_layers=args.num_layers,
-                      dropout=args.dropout)
+                      dropout=args.dropout, **model_options(args))
     own = partition_from_chunks(args.data_path, args.graph_name, args.part_method, args.n_part, rank, meta.n_dim,
                                 device)
     tr = FullGraphTrainer(model, own, lr=args.lr, repart_every=args.repart_every, comm=Comm() if world > 1 else None,
-                          seed=args.seed)
+                          seed=args.seed, act_bits=args.act_bits)
     losses = []
     for epoch in range(args.num_epochs):
         tic = time.time()

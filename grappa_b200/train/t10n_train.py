@@ -136,6 +136,13 @@ def save_to_ckpt(args, epoch, rank, model, optimizer_state, loss):
     return name
 
 
+def model_options(args):
+    """get_model's options of the command line (GraphSAGE's layer form)."""
+    if args.act_bits != 16 and args.num_gpus == -1:
+        raise ValueError("--act_bits 8 keeps activations in 8 bits on the GPU; CPU training has 32")
+    return dict(activation=args.activation, norm=None if args.norm == "none" else args.norm, residual=args.residual)
+
+
 def run_cpu(args):
     """CPU ranks: the reference's training loop on the host engine."""
     from grappa_b200.dataloader import IsolatedDataloader
@@ -145,7 +152,7 @@ def run_cpu(args):
     meta = name_to_meta(args.graph_name)
     torch.manual_seed(args.seed)
     model = get_model(args.model, meta.n_dim, meta.n_label, num_hidden=args.num_hidden, num_layers=args.num_layers,
-                      dropout=args.dropout)
+                      dropout=args.dropout, **model_options(args))
     optimizer = torch.optim.Adam(model.parameters(), lr=args.lr)
     ckpt_epoch = resume_from_ckpt(model, optimizer, resilience.resolve_resume(args))
     loader = IsolatedDataloader(device, args)
@@ -259,7 +266,7 @@ def run_gpu(args):
     meta = name_to_meta(args.graph_name)
     torch.manual_seed(args.seed)
     model = get_model(args.model, meta.n_dim, meta.n_label, num_hidden=args.num_hidden, num_layers=args.num_layers,
-                      dropout=args.dropout)
+                      dropout=args.dropout, **model_options(args))
     ckpt = None
     resume = resilience.resolve_resume(args)
     if resume:
@@ -270,7 +277,7 @@ def run_gpu(args):
     comm = Comm() if world > 1 else None
     fanouts = [int(f) for f in args.fan_out.split(",")]
     trainer = MiniBatchTrainer(model, own, fanouts, args.batch_size, lr=args.lr, repart_every=args.repart_every,
-                               comm=comm, seed=args.seed)
+                               comm=comm, seed=args.seed, act_bits=args.act_bits)
     if ckpt is not None:
         trainer.engine.load_optimizer_state_dict(ckpt["optimizer_state_dict"])
     first = int(ckpt["epoch"]) + 1 if ckpt is not None else 0
@@ -343,6 +350,12 @@ def build_parser():
     p.add_argument("--batch_size_eval", type=int, default=100000)
     p.add_argument("--lr", type=float, default=0.003)
     p.add_argument("--dropout", type=float, default=0.5)
+    p.add_argument("--activation", type=str, default="relu", choices=["relu", "gelu", "silu"], help="sage: activation")
+    p.add_argument("--norm", type=str, default="none", choices=["none", "rms"],
+                   help="sage: RMS norm before every layer but the first")
+    p.add_argument("--residual", action="store_true", help="sage: residual hidden layers (with --norm rms)")
+    p.add_argument("--act_bits", type=int, default=16, choices=[8, 16],
+                   help="sage on GPUs: bits of the activations kept for the backward pass")
     p.add_argument("--stop_at_border", action="store_true", default=False, help="sampler will stop at border")
     p.add_argument("--disable_backup_server", action="store_true", default=False)
     p.add_argument("--repart_every", type=int, default=50)

@@ -10,6 +10,8 @@
   * seeds are reshuffled every epoch;
   * gradients are aggregated with the coverage-corrected all-reduce.
 
+``act_bits=8`` (GraphSAGE) keeps what the backward pass reads in 8 bits.
+
 Seeds can be fed from device memory (``host_feed=False``) or, as a user with data
 on the host would, from pinned host memory with the loss read back every step
 (``host_feed=True``).
@@ -26,7 +28,7 @@ from grappa_b200.graph_store import PartitionStore, next_neighbor
 
 class MiniBatchTrainer:
     def __init__(self, model, own, fanouts, batch_size, lr=3e-3, repart_every=10, comm=None, seed=0,
-                 fused_allreduce=True, use_cuda_graph=True, ar_mode=None, overlap_allreduce=True):
+                 fused_allreduce=True, use_cuda_graph=True, ar_mode=None, overlap_allreduce=True, act_bits=16):
         self.model = model
         self.own = own
         self.comm = comm
@@ -50,7 +52,7 @@ class MiniBatchTrainer:
         self.engine = make_engine(model, self.store.cap_nodes, fanouts, self.batch_size, self.device, lr=lr,
                                  comm=comm, seed=seed, fused_allreduce=fused_allreduce,
                                  use_cuda_graph=use_cuda_graph, ar_mode=ar_mode,
-                                 overlap_allreduce=overlap_allreduce)
+                                 overlap_allreduce=overlap_allreduce, act_bits=act_bits)
         self._maybe_repartition(0)
         self._warm = False
 
@@ -278,7 +280,7 @@ class FullGraphTrainer:
     (training, validation and test); here only the training nodes contribute."""
 
     def __init__(self, model, own, lr=3e-3, repart_every=10, comm=None, seed=0, fused_allreduce=True,
-                 use_cuda_graph=True, ar_mode=None):
+                 use_cuda_graph=True, ar_mode=None, act_bits=16):
         from grappa_b200.engine import make_engine
 
         self.model, self.own, self.comm = model, own, comm
@@ -297,7 +299,7 @@ class FullGraphTrainer:
         blocks = full_graph_blocks(w, len(model.layers), own, *self._caps)
         self.engine = make_engine(model, self.store.cap_nodes, [], 0, self.device, lr=lr, comm=comm, seed=seed,
                                   fused_allreduce=fused_allreduce, use_cuda_graph=use_cuda_graph, blocks=blocks,
-                                  ar_mode=ar_mode)
+                                  ar_mode=ar_mode, act_bits=act_bits)
         self.engine.bind_working(w, own.label, own.gideg)
         self._last_repart = 0
         self._warm = False
