@@ -295,6 +295,7 @@ void linear_fwd(Tensor A, Tensor W, OptT n_dev, int64_t cap, Tensor out, Tensor 
   }
   std::vector<Mat> coded;
   a.q8 = rows8(q, q_exp, cap, N, kWrite, &coded);
+  if (!coded.empty()) a.q_rows = coded[0].rows;
   for (const Mat& m : coded) {
     all_apart(m, others);
     apart(m, mr);

@@ -575,9 +575,14 @@ struct LinearArgs {
   __nv_bfloat16* z = nullptr;
   int64_t ldz = 0;
   Rows8 q8;
+  int64_t q_rows = 0;
   int32_t* err = nullptr;
 };
 void launch_linear_fwd(const LinearArgs& a, cudaStream_t stream);
+// its tile shapes: 256 columns by CTA pairs, 128 and 64 columns by single CTAs
+void launch_linear_pair(const LinearArgs& a, cudaStream_t stream);
+void launch_linear_128(const LinearArgs& a, cudaStream_t stream);
+void launch_linear_64(const LinearArgs& a, cudaStream_t stream);
 
 // dz = dropout mask(dout) act'(z), dbias (+)= column sums of dz (before its rounding);
 // rows [n, roundup(n, 64)) of dz below cap are zeroed (the weight-gradient GEMM reads
