@@ -130,6 +130,12 @@ __device__ __forceinline__ void mask8(float* v, int c, int dim) {
     if (c * 8 + i >= dim) v[i] = 0.f;
 }
 
+// the first n of eight bf16 columns, zeros after them
+__device__ __forceinline__ uint4 first_columns(uint4 o, int n) {
+  auto keep = [](uint32_t w, int k) { return k >= 2 ? w : (k == 1 ? w & 0xFFFFu : 0u); };
+  return make_uint4(keep(o.x, n), keep(o.y, n - 2), keep(o.z, n - 4), keep(o.w, n - 6));
+}
+
 __device__ __forceinline__ int live_rows(const int32_t* n_ptr, int cap) {
   return n_ptr ? max(0, min(*n_ptr, cap)) : cap;
 }

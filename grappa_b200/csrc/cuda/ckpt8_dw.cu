@@ -49,7 +49,7 @@ struct DSmem {
   static constexpr int kSlots = kBudget / kSlotBytes > 12 ? 12 : kBudget / kSlotBytes;
   static constexpr int kTmemCols = MT * NT;
   static constexpr int kBytes = kSlots * kSlotBytes + kBSlots * kBBytes + 1024 /*align*/;
-  static_assert(kSlots >= 3 && kTmemCols <= 512 && kBytes <= 226 * 1024, "ckpt8_dw: shared memory");
+  static_assert(kSlots >= kTeams && kTmemCols <= 512 && kBytes <= 226 * 1024, "ckpt8_dw: shared memory");
 };
 
 // How the rows are shared: kb_total blocks of BK rows over `splits` CTAs a tile, fewer
@@ -68,7 +68,9 @@ __host__ __device__ inline Shares shares(int kb_total, int splits_max, int min_k
 struct DwPlan {
   int mt, nt;            // tile: 128 mt x nt
   int m_tiles, n_tiles;
-  int splits, min_kb;
+  int rows;              // of a block
+  int splits, min_kb;    // CTAs (pairs) a tile at most, blocks each at least
+  bool pair = false;     // by CTA pairs (mt = 2, nt = 256)
   bool y_blocks = false, q_blocks = false;  // operands of whole column blocks (64 bf16, 128 codes)
 };
 
@@ -220,8 +222,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; i < end; i += kTeams) {
         const int s = i % kSlots;
         const int r0 = (kb0 + i) * BK;
-        bool ok = mbar_wait(&full_bar[s], (i / kSlots) & 1u, &abort_flag);
-        if (ok && i >= kTeams) ok = mbar_wait(&b_empty[b], (i / kTeams - 1) & 1u, &abort_flag);
+        // the operand slot first: its last block's products are done, so block i - kSlots has
+        // come (a wait by parity must not begin two phases early, and loads may complete out
+        // of order)
+        bool ok = i < kTeams || mbar_wait(&b_empty[b], (i / kTeams - 1) & 1u, &abort_flag);
+        ok = ok && mbar_wait(&full_bar[s], (i / kSlots) & 1u, &abort_flag);
         if (!ok) {
           if (lane == 0) set_error(a.err, kErrMmaTimeout);
           abort_flag = 1;
@@ -303,35 +308,312 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// gW (+)= the partial tiles of the splits, in order.  One thread per four columns of a row
-// of a tile, in the partial tiles' own order.
+// ---------------------------------------------------------------- CTA pairs
+// The large tile (256 x 256) by two CTAs (cta_group::2): each loads 128 columns of dY and
+// 128 columns of codes, converts its own, and the products read both CTAs' operands.  Per
+// SM that halves the operand bytes that the tensor core reads from shared memory (which
+// bound the single CTA: 96 KB of traffic a 32-row block against 512 cycles of products),
+// and the accumulator takes half of TMEM, so there are two: four warps of their own empty
+// one while the products of the next 4096 rows fill the other.
+//   warp 0        TMA producer of dY: 128 columns a CTA, on CTA 0's barrier
+//   warp 1        (CTA 0) issues the products
+//   warp 2        TMA producer of the codes, on the CTA's own barriers
+//   warps 3..10   converters, two warps (32 rows each) a block, one pair of them for every
+//                 slot of the codes' ring
+//   warps 11..14  epilogue
+// A slot holds a block's dY (64 rows) and its converted rows, and one commit to both CTAs
+// frees both; the codes have a shorter ring of their own that the converters free, so that
+// the way from a free slot to its products is the longer of a load and a conversion, not
+// their sum (the slots' turn bounds the rate: 4100 cycles over 5 slots with the codes in
+// the slot).  The last block of a partly filled 64 rows takes its dY through the
+// converters, which write zeros for the rows past the live ones.
+struct PairSmem {
+  static constexpr int kRows = 64;
+  static constexpr int kYBytes = 128 * kRows * 2;
+  static constexpr int kBBytes = 128 * kRows * 2;
+  static constexpr int kQBytes = 128 * kRows;
+  static constexpr int kSlotBytes = kYBytes + kBBytes;
+  static constexpr int kSlots = 6;
+  static constexpr int kQSlots = 4;
+  static constexpr int kWarps = 3 + 2 * kQSlots + 4;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kChain = kChainRows / kRows;
+  static constexpr int kBytes = kSlots * kSlotBytes + kQSlots * kQBytes + 1024 /*align*/;
+  static_assert(kBytes <= 226 * 1024, "ckpt8_dw pair: shared memory");
+};
+
+__global__ void __launch_bounds__(PairSmem::kThreads, 1)
+    ckpt8_dw_pair_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmQ,
+                         Ckpt8DwArgs a, DwPlan plan) {
+  GB_PDL_ENTRY();
+  using S = PairSmem;
+  constexpr int kSlots = S::kSlots, kQSlots = S::kQSlots, kRows = S::kRows, kChain = S::kChain;
+  constexpr int NT = 256;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t y_full[kSlots], done_bar[kSlots], b_full[kSlots], q_full[kQSlots], q_empty[kQSlots], acc_full[2],
+      acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  const int n = live_rows(a.n_ptr, a.cap);
+  const int kb_total = (n + kRows - 1) / kRows;
+  const Shares sh = shares(kb_total, plan.splits, plan.min_kb);
+  const int pair = blockIdx.x >> 1, rank = static_cast<int>(cluster_rank());
+  const int tile = pair % (plan.m_tiles * plan.n_tiles), split = pair / (plan.m_tiles * plan.n_tiles);
+  if (split >= sh.splits) return;  // both CTAs of the pair
+  const int m0 = (tile / plan.n_tiles) * 256 + rank * 128, n0 = (tile % plan.n_tiles) * NT + rank * 128;
+  const int kb0 = split * sh.per, nkb = max(0, min(kb_total, kb0 + sh.per) - kb0);
+  // local number of the partly filled block (-1: none here)
+  const int tail = n % kRows != 0 && kb0 + nkb == kb_total ? nkb - 1 : -1;
+  float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * NT);
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_area = smem + kSlots * S::kSlotBytes;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&y_full[s], 1);
+      mbar_init(&done_bar[s], 1);
+      mbar_init(&b_full[s], 4);  // the block's two converters in either CTA
+    }
+    for (int s = 0; s < kQSlots; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 2);  // the block's two converters
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8);  // four warps in either CTA
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * NT);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % kSlots;
+        if (i >= kSlots && !mbar_wait(&done_bar[s], ((i / kSlots) & 1u) ^ 1u, &abort_flag)) {
+          set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          break;
+        }
+        if (i == tail) {
+          if (rank == 0) mbar_arrive(&y_full[s]);
+          continue;
+        }
+        uint8_t* sy = smem + s * S::kSlotBytes;
+        const int r0 = (kb0 + i) * kRows;
+        if (rank == 0) mbar_expect_tx(&y_full[s], 2 * S::kYBytes);
+        const uint32_t bar = cluster_addr(&y_full[s], 0);
+        tma_load_2d_pair(sy, &tmY, bar, m0, r0);
+        tma_load_2d_pair(sy + 64 * kRows * 2, &tmY, bar, m0 + 64, r0);
+        issued = i + 1;
+      }
+      if (abort_flag && rank == 0) {
+        for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(&y_full[i % kSlots], (i / kSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = umma_idesc(256, NT, true, true);
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % kSlots;
+        const int chain = i / kChain, ab = chain & 1;
+        const bool first = i % kChain == 0;
+        if ((first && chain >= 2 && !mbar_wait(&acc_empty[ab], ((chain >> 1) - 1) & 1u, &abort_flag)) ||
+            !mbar_wait(&y_full[s], (i / kSlots) & 1u, &abort_flag) ||
+            !mbar_wait(&b_full[s], (i / kSlots) & 1u, &abort_flag)) {
+          set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sy = smem_u32(smem + s * S::kSlotBytes), sb = sy + S::kYBytes;
+#pragma unroll
+        for (int kk = 0; kk < kRows / 16; ++kk)
+          umma_f16_pair(tmem_base + ab * NT, umma_desc(sy + kk * 2048, 64 * kRows * 2, 1024),
+                        umma_desc(sb + kk * 2048, 64 * kRows * 2, 1024), idesc, (!first || kk > 0) ? 1u : 0u);
+        umma_commit_pair(&done_bar[s]);
+        if (i % kChain == kChain - 1 || i == nkb - 1) umma_commit_pair(&acc_full[ab]);
+      }
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % kQSlots;
+        if (i >= kQSlots && !mbar_wait(&q_empty[s], ((i / kQSlots) & 1u) ^ 1u, &abort_flag)) {
+          set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          break;
+        }
+        mbar_expect_tx(&q_full[s], S::kQBytes);
+        tma_load_2d(q_area + s * S::kQBytes, &tmQ, &q_full[s], n0, (kb0 + i) * kRows);
+        issued = i + 1;
+      }
+      if (abort_flag) {
+        for (int i = issued > kQSlots ? issued - kQSlots : 0; i < issued; ++i) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(&q_full[i % kQSlots], (i / kQSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
+          }
+        }
+      }
+    }
+  } else if (warp < 3 + 2 * kQSlots) {
+    // A pair of warps keeps to one slot of the codes' ring and takes its blocks in order, so
+    // its wait by parity never begins two phases early; the same holds for the wait on
+    // done_bar, since block i - kQSlots was converted after block i - kQSlots - kSlots's products.
+    const int qs = (warp - 3) >> 1, k = ((warp - 3) & 1) * 32 + lane;  // code slot, row of the block
+    const uint8_t* row = q_area + qs * S::kQBytes + k * 128;
+    uint32_t byte[kAhead][4];
+    auto fetch = [&](int i, uint32_t (&to)[4]) {
+      const int r = (kb0 + i) * kRows + k;
+      const uint8_t* e = a.q8.e + static_cast<int64_t>(r) * a.q8.lde + n0 / 32;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) to[u] = (i < nkb && r < n && n0 / 32 + u < a.groups) ? __ldg(e + u) : 0u;
+    };
+#pragma unroll
+    for (int p = 0; p < kAhead; ++p) fetch(qs + kQSlots * p, byte[p]);
+    for (int i = qs; i < nkb; i += kQSlots) {
+      const int r0 = (kb0 + i) * kRows, s = i % kSlots;
+      uint8_t* sy = smem + s * S::kSlotBytes;
+      uint8_t* sb = sy + S::kYBytes;
+      bool ok = mbar_wait(&q_full[qs], (i / kQSlots) & 1u, &abort_flag);
+      if (ok && i >= kSlots) ok = mbar_wait(&done_bar[s], (i / kSlots - 1) & 1u, &abort_flag);
+      if (!ok) {
+        if (lane == 0) set_error(a.err, kErrMmaTimeout);
+        abort_flag = 1;
+        break;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const __nv_bfloat162 scale = group8_scale_bf16(byte[0][u]);
+        uint8_t* out = sb + (u >> 1) * (64 * kRows * 2) + k * 128;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 c = *reinterpret_cast<const uint4*>(row + (((u * 2 + h) ^ (k & 7)) << 4));
+          uint4 v0 = values8_bf16(c.x, c.y, scale), v1 = values8_bf16(c.z, c.w, scale);
+          if (r0 + k >= n) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(out + ((((u & 1) * 4 + h * 2) ^ (k & 7)) << 4)) = v0;
+          *reinterpret_cast<uint4*>(out + ((((u & 1) * 4 + h * 2 + 1) ^ (k & 7)) << 4)) = v1;
+        }
+      }
+      if (i == tail) {
+        // dY's rows by plain loads (16 pieces of 8 columns), zeros past the live rows
+        const __nv_bfloat16* y = a.dy + static_cast<int64_t>(r0 + k) * a.lddy + m0;
+#pragma unroll 1
+        for (int p = 0; p < 16; ++p) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (r0 + k < n && m0 + 8 * p < a.M) v = first_columns(*reinterpret_cast<const uint4*>(y + 8 * p), a.M - m0 - 8 * p);
+          *reinterpret_cast<uint4*>(sy + (p >> 3) * (64 * kRows * 2) + k * 128 + (((p & 7) ^ (k & 7)) << 4)) = v;
+        }
+      }
+#pragma unroll
+      for (int p = 0; p + 1 < kAhead; ++p)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) byte[p][u] = byte[p + 1][u];
+      fetch(i + kQSlots * kAhead, byte[kAhead - 1]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&q_empty[qs]);
+        mbar_arrive_cluster(cluster_addr(&b_full[s], 0));
+      }
+    }
+  } else {
+    // epilogue: warp w drains TMEM lanes of its quarter into the CTA's partial tile, laid out
+    // as in ckpt8_dw_kernel
+    const int quarter = warp & 3;
+    for (int chain = 0; chain * kChain < nkb; ++chain) {
+      const int ab = chain & 1;
+      if (!mbar_wait(&acc_full[ab], (chain >> 1) & 1u, &abort_flag)) {
+        if (lane == 0) set_error(a.err, kErrMmaTimeout);
+        abort_flag = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+      for (int c = 0; c < NT; c += 32) {
+        float v[32];
+        tmem_ld32(tmem_base + static_cast<uint32_t>(ab * NT + c) + (static_cast<uint32_t>(quarter * 32) << 16), v);
+        float* p = part + (static_cast<int64_t>(c / 32) * 4 + quarter) * 1024 + lane * 4;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (chain == 0)
+            *reinterpret_cast<float4*>(p + j * 128) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          else
+            red_add_v4(p + j * 128, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[ab], 0));
+    }
+  }
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still use its memory or barriers
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    tmem_dealloc_pair(tmem_base, 2 * NT);
+  }
+}
+
+// gW (+)= the partial tiles of the splits.  A thread takes four columns of a row of a tile (in
+// the partial tiles' own order) and a fourth of the splits, in order; the four shares are
+// joined in order through shared memory.
 __global__ void __launch_bounds__(256) ckpt8_dw_sum_kernel(Ckpt8DwArgs a, DwPlan plan) {
   GB_PDL_ENTRY();
+  __shared__ float4 sh4[4][64];
   const int n = live_rows(a.n_ptr, a.cap);
-  const int kb_total = (n + BK - 1) / BK;
+  const int kb_total = (n + plan.rows - 1) / plan.rows;
   const int splits = kb_total > 0 ? shares(kb_total, plan.splits, plan.min_kb).splits : 0;
   const int tile_floats = 128 * plan.mt * plan.nt;
   const int tiles = plan.m_tiles * plan.n_tiles;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int x = threadIdx.x & 63, share = threadIdx.x >> 6;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + x;  // the grid covers the tiles exactly
   const int tile = static_cast<int>(i / (tile_floats / 4));
-  if (tile >= tiles) return;
   const int at = static_cast<int>(i % (tile_floats / 4)) * 4;
-  // at = ((c / 32) * 4 + quarter) * 1024 + j * 128 + lane * 4
-  const int lane = (at / 4) % 32, j = (at / 128) % 8, quarter = (at / 1024) % 4, c32 = at / 4096;
-  const int col_t = c32 * 32 + j * 4;  // column over the MT accumulators
-  const int m = (tile / plan.n_tiles) * 128 * plan.mt + (col_t / plan.nt) * 128 + quarter * 32 + lane;
-  const int nn = (tile % plan.n_tiles) * plan.nt + col_t % plan.nt;
-  if (m >= a.M || nn >= a.N) return;
+  const int per = (splits + 3) / 4, k1 = min(splits, (share + 1) * per);
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   const float* p = a.work + static_cast<int64_t>(tile) * tile_floats + at;
 #pragma unroll 8
-  for (int k = 0; k < splits; ++k) {
+  for (int k = share * per; k < k1; ++k) {
     const float4 v = *reinterpret_cast<const float4*>(p + static_cast<int64_t>(k) * tiles * tile_floats);
     s.x += v.x;
     s.y += v.y;
     s.z += v.z;
     s.w += v.w;
   }
+  sh4[share][x] = s;
+  __syncthreads();
+  if (share != 0) return;
+#pragma unroll
+  for (int q = 1; q < 4; ++q) {
+    const float4 v = sh4[q][x];
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
+  }
+  // at = ((c / 32) * 4 + quarter) * 1024 + j * 128 + lane * 4
+  const int lane = (at / 4) % 32, j = (at / 128) % 8, quarter = (at / 1024) % 4, c32 = at / 4096;
+  const int col_t = c32 * 32 + j * 4;  // column over the MT accumulators
+  const int m = (tile / plan.n_tiles) * 128 * plan.mt + (col_t / plan.nt) * 128 + quarter * 32 + lane;
+  const int nn = (tile % plan.n_tiles) * plan.nt + col_t % plan.nt;
+  if (m >= a.M || nn >= a.N) return;
   float* g = a.gw + static_cast<int64_t>(m) * a.ldg + nn;
   const float o[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -345,7 +627,8 @@ __global__ void __launch_bounds__(256) ckpt8_dw_sum_kernel(Ckpt8DwArgs a, DwPlan
 // spreads the same work over four times as many CTAs.
 DwPlan plan_for(int M, int N, int cap, int num_sms) {
   DwPlan p;
-  const int64_t kb = ceil_div(std::max(cap, 1), BK);
+  int64_t kb = ceil_div(std::max(cap, 1), BK);
+  p.rows = BK;
   p.mt = M > 128 ? 2 : 1;
   p.nt = N > 128 ? 256 : 128;
   p.min_kb = 16;
@@ -356,26 +639,49 @@ DwPlan plan_for(int M, int N, int cap, int num_sms) {
   }
   p.m_tiles = static_cast<int>(ceil_div(M, 128 * p.mt));
   p.n_tiles = static_cast<int>(ceil_div(N, p.nt));
+  p.pair = p.mt == 2 && p.nt == 256;
+  if (p.pair) {
+    p.rows = PairSmem::kRows;
+    p.min_kb = 8;
+    kb = ceil_div(std::max(cap, 1), p.rows);
+  }
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms / tiles, kb / p.min_kb)));
+  const int64_t at_once = p.pair ? num_sms / 2 : num_sms;
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(at_once / tiles, kb / p.min_kb)));
   return p;
+}
+
+CUtensorMap map_y(const Ckpt8DwArgs& a, const DwPlan& p, int rows, int blocks) {
+  return p.y_blocks ? tensor_map_blocks(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.dy, a.dy_rows, a.dy_cols, a.lddy, 64, rows,
+                                        blocks)
+                    : tensor_map_bf16(a.dy, a.dy_rows, a.dy_cols, a.lddy, rows);
+}
+CUtensorMap map_q(const Ckpt8DwArgs& a, int rows) {
+  return tensor_map_u8(a.q8.q, a.q_rows, a.q_cols, a.q8.ldq, 128, rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int MT, int NT>
 void launch_t(const Ckpt8DwArgs& a, DwPlan p, cudaStream_t stream) {
   using S = DSmem<MT, NT>;
   p.y_blocks = a.dy_cols % 64 == 0;
-  p.q_blocks = a.q_cols % 128 == 0;
-  const CUtensorMap my = p.y_blocks ? tensor_map_blocks(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.dy, a.dy_rows, a.dy_cols,
-                                                        a.lddy, 64, BK, 2 * MT)
-                                    : tensor_map_bf16(a.dy, a.dy_rows, a.dy_cols, a.lddy, BK);
-  const CUtensorMap mq =
-      p.q_blocks ? tensor_map_blocks(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.q8.q, a.q_rows, a.q_cols, a.q8.ldq, 128, BK, NT / 128)
-                 : tensor_map_u8(a.q8.q, a.q_rows, a.q_cols, a.q8.ldq, 128, BK, CU_TENSOR_MAP_SWIZZLE_128B);
+  p.q_blocks = NT > 128 && a.q_cols % 128 == 0;
+  const CUtensorMap my = map_y(a, p, BK, 2 * MT);
+  const CUtensorMap mq = p.q_blocks ? tensor_map_blocks(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.q8.q, a.q_rows, a.q_cols,
+                                                        a.q8.ldq, 128, BK, NT / 128)
+                                    : map_q(a, BK);
   auto kern = ckpt8_dw_kernel<MT, NT>;
   set_smem(reinterpret_cast<const void*>(kern), S::kBytes);
   launch_k(kern, dim3(static_cast<unsigned>(p.m_tiles * p.n_tiles * p.splits)), dim3(kThreads), S::kBytes, stream, my,
            mq, a, p);
+  GB_LAUNCH_CHECK();
+}
+
+void launch_pair(const Ckpt8DwArgs& a, DwPlan p, cudaStream_t stream) {
+  using S = PairSmem;
+  const CUtensorMap my = tensor_map_bf16(a.dy, a.dy_rows, a.dy_cols, a.lddy, S::kRows), mq = map_q(a, S::kRows);
+  set_smem(reinterpret_cast<const void*>(ckpt8_dw_pair_kernel), S::kBytes);
+  launch_cluster_k(ckpt8_dw_pair_kernel, dim3(static_cast<unsigned>(p.m_tiles * p.n_tiles * p.splits * 2)),
+                   dim3(S::kThreads), 2, S::kBytes, stream, my, mq, a, p);
   GB_LAUNCH_CHECK();
 }
 
@@ -388,12 +694,14 @@ int64_t ckpt8_dw_work_floats(int M, int N, int cap, int num_sms) {
 
 void launch_ckpt8_dw(const Ckpt8DwArgs& a, int num_sms, cudaStream_t stream) {
   const DwPlan p = plan_for(a.M, a.N, a.cap, num_sms);
-  if (p.mt == 2)
-    p.nt == 256 ? launch_t<2, 256>(a, p, stream) : launch_t<2, 128>(a, p, stream);
+  if (p.pair)
+    launch_pair(a, p, stream);
+  else if (p.mt == 2)
+    launch_t<2, 128>(a, p, stream);
   else
     p.nt == 256 ? launch_t<1, 256>(a, p, stream) : launch_t<1, 128>(a, p, stream);
   const int64_t threads = static_cast<int64_t>(p.m_tiles) * p.n_tiles * 128 * p.mt * p.nt / 4;
-  launch_k(ckpt8_dw_sum_kernel, dim3(static_cast<unsigned>(ceil_div(threads, 256))), dim3(256), 0, stream, a, p);
+  launch_k(ckpt8_dw_sum_kernel, dim3(static_cast<unsigned>(threads / 64)), dim3(256), 0, stream, a, p);
   GB_LAUNCH_CHECK();
 }
 

@@ -73,12 +73,6 @@ __device__ __forceinline__ uint2 codes8_relu(const float* v, float inv) {
   return q;
 }
 
-// the first n of eight bf16 columns, zeros after them
-__device__ __forceinline__ uint4 first_columns(uint4 o, int n) {
-  auto keep = [](uint32_t w, int k) { return k >= 2 ? w : (k == 1 ? w & 0xFFFFu : 0u); };
-  return make_uint4(keep(o.x, n), keep(o.y, n - 2), keep(o.z, n - 4), keep(o.w, n - 6));
-}
-
 template <int BN, int CG, int ACT, bool RES, bool Q8, bool ANY>
 __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
     linear_fwd_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
@@ -184,9 +178,7 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
         const int b = lt & 1;
         if (lt >= 2) {
           const uint32_t parity = ((lt >> 1) - 1) & 1u;
-          const bool ok = CG == 2 ? mbar_wait_cluster(&acc_empty[b], parity, &abort_flag)
-                                  : mbar_wait(&acc_empty[b], parity, &abort_flag);
-          if (!ok) {
+          if (!mbar_wait(&acc_empty[b], parity, &abort_flag)) {
             set_error(a.err, kErrMmaTimeout);
             abort_flag = 1;
             break;

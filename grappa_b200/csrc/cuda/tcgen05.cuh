@@ -193,27 +193,30 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
       "h"(static_cast<uint16_t>(3))
       : "memory");
 }
+// Arrives on a barrier of the other (or this) CTA of the cluster.  What it hands over is
+// tensor memory that has been read (tcgen05.wait::ld and the fence before it) or shared
+// memory written through fence.proxy.async, so the default scope is enough on both sides;
+// with .release.cluster here and .acquire.cluster on the wait, every hand-over also waited
+// for the warp's global stores (measured: the weight gradient 286 us instead of PAIR_US).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// mbar_wait on a barrier that the other CTA arrives on
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+
+// mbar_wait that polls without suspending the thread
+__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   uint64_t t0 = 0;
   for (;;) {
-    // the timer is read after the first polls only: an ordinary wait ends before
-    for (int i = 0; i < 256; ++i)
-      if (mbar_try_wait_cluster(bar, parity)) return true;
+    for (int i = 0; i < 1024; ++i) {
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(smem_u32(bar)), "r"(parity)
+          : "memory");
+      if (ok) return true;
+    }
     if (*abort_flag) return false;
     const uint64_t now = globaltimer_ns();
     if (t0 == 0) t0 = now;

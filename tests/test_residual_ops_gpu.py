@@ -463,7 +463,10 @@ def test_linear_act_bwd_draws_the_forward_mask():
 @pytest.mark.parametrize("n,cap,k,m", [(1, 1, 1, 1), (5, 9, 8, 8), (63, 64, 100, 47), (64, 64, 32, 128), (65, 200, 130, 129),
                                        (1000, 3000, 208, 256), (3250, 10240, 512, 256), (4097, 4100, 264, 40),
                                        (40000, 40000, 96, 200), (150001, 150016, 136, 64), (0, 64, 40, 40),
-                                       (2048, 2048, 1000, 300)])
+                                       (2048, 2048, 1000, 300),
+                                       # enough rows for the 256 x 256 tiles of CTA pairs
+                                       (40003, 40100, 300, 300), (152064, 152064, 512, 256), (160001, 170000, 136, 200),
+                                       (40960, 41000, 520, 264)])
 @pytest.mark.parametrize("wide", [0, 64])
 def test_ckpt8_dw(n, cap, k, m, wide):
     g = gen_for("dw", n, k, m)
