@@ -121,19 +121,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = tmem_slot;
   const int nkb = max(0, kb1 - kb0);
 
+  // the two issuing warps stay converged; one elected lane issues (elect_one)
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % kSlots;
-        if (i >= kSlots && !mbar_wait(&empty_bar[s], ((i / kSlots) & 1u) ^ 1u, &abort_flag)) {
-          set_error(a.err, kErrMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        uint8_t* sa = smem + s * S::kSlotBytes;
-        uint8_t* sq = sa + S::kABytes;
-        const int r0 = (kb0 + i) * BK;
+    int issued = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % kSlots;
+      if (i >= kSlots && !mbar_wait_all(&empty_bar[s], ((i / kSlots) & 1u) ^ 1u, &abort_flag)) {
+        if (lane == 0) set_error(a.err, kErrMmaTimeout);
+        abort_flag = 1;
+        break;
+      }
+      uint8_t* sa = smem + s * S::kSlotBytes;
+      uint8_t* sq = sa + S::kABytes;
+      const int r0 = (kb0 + i) * BK;
+      if (elect_one()) {
         mbar_expect_tx(&full_bar[s], S::kSlotBytes);
         // whole column blocks: one load an operand
         if (plan.y_blocks) {
@@ -148,38 +149,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < NT / 128; ++c) tma_load_2d(sq + c * (128 * BK), &tmQ, &full_bar[s], n0 + c * 128, r0);
         }
-        issued = i + 1;
       }
-      if (abort_flag) {
-        for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&full_bar[i % kSlots], (i / kSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
-          }
+      __syncwarp();
+      issued = i + 1;
+    }
+    if (abort_flag) {
+      for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&full_bar[i % kSlots], (i / kSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc(128, NT, true, true);
-      int chunk = 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % kSlots, b = i % kTeams;
-        const bool first = i % kChainKb == 0;
-        // the accumulator of the last chain has been read
-        if (first && chunk > 0 && !mbar_wait(&acc_empty, (chunk - 1) & 1u, &abort_flag)) {
-          set_error(a.err, kErrMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        // dY's tile (the loads' own barrier) and the converted rows
-        if (!mbar_wait(&full_bar[s], (i / kSlots) & 1u, &abort_flag) ||
-            !mbar_wait(&b_full[b], (i / kTeams) & 1u, &abort_flag)) {
-          set_error(a.err, kErrMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t sa = smem_u32(smem + s * S::kSlotBytes), sb = smem_u32(b_area + b * S::kBBytes);
+    constexpr uint32_t idesc = umma_idesc(128, NT, true, true);
+    int chunk = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % kSlots, b = i % kTeams;
+      const bool first = i % kChainKb == 0;
+      // the accumulator of the last chain has been read; dY's tile (the loads' own barrier)
+      // and the converted rows have come
+      if ((first && chunk > 0 && !mbar_wait_all(&acc_empty, (chunk - 1) & 1u, &abort_flag)) ||
+          !mbar_wait_all(&full_bar[s], (i / kSlots) & 1u, &abort_flag) ||
+          !mbar_wait_all(&b_full[b], (i / kTeams) & 1u, &abort_flag)) {
+        if (lane == 0) set_error(a.err, kErrMmaTimeout);
+        abort_flag = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t sa = smem_u32(smem + s * S::kSlotBytes), sb = smem_u32(b_area + b * S::kBBytes);
+      const bool last = i % kChainKb == kChainKb - 1 || i == nkb - 1;
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk) {
           const uint64_t db = umma_desc(sb + kk * 2048, 64 * BK * 2, 1024);
@@ -190,11 +189,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         umma_commit(&empty_bar[s]);
         umma_commit(&b_empty[b]);
-        if (i % kChainKb == kChainKb - 1 || i == nkb - 1) {
-          umma_commit(&acc_full);
-          ++chunk;
-        }
+        if (last) umma_commit(&acc_full);
       }
+      __syncwarp();
+      if (last) ++chunk;
     }
   } else {
     // the teams take the blocks in turn, each with an operand slot of its own: a team has four
@@ -225,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the operand slot first: its last block's products are done, so block i - kSlots has
         // come (a wait by parity must not begin two phases early, and loads may complete out
         // of order)
-        bool ok = i < kTeams || mbar_wait(&b_empty[b], (i / kTeams - 1) & 1u, &abort_flag);
-        ok = ok && mbar_wait(&full_bar[s], (i / kSlots) & 1u, &abort_flag);
+        bool ok = i < kTeams || mbar_wait_all(&b_empty[b], (i / kTeams - 1) & 1u, &abort_flag);
+        ok = ok && mbar_wait_all(&full_bar[s], (i / kSlots) & 1u, &abort_flag);
         if (!ok) {
           if (lane == 0) set_error(a.err, kErrMmaTimeout);
           abort_flag = 1;
@@ -273,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&b_full[b]);
       }
       if (stop) break;
-      if (!mbar_wait(&acc_full, chunk & 1u, &abort_flag)) {
+      if (!mbar_wait_all(&acc_full, chunk & 1u, &abort_flag)) {
         if (lane == 0) set_error(a.err, kErrMmaTimeout);
         abort_flag = 1;
         break;
@@ -318,28 +316,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 //   warp 0        TMA producer of dY: 128 columns a CTA, on CTA 0's barrier
 //   warp 1        (CTA 0) issues the products
 //   warp 2        TMA producer of the codes, on the CTA's own barriers
-//   warps 3..10   converters, two warps (32 rows each) a block, one pair of them for every
-//                 slot of the codes' ring
-//   warps 11..14  epilogue
-// A slot holds a block's dY (64 rows) and its converted rows, and one commit to both CTAs
-// frees both; the codes have a shorter ring of their own that the converters free, so that
-// the way from a free slot to its products is the longer of a load and a conversion, not
-// their sum (the slots' turn bounds the rate: 4100 cycles over 5 slots with the codes in
-// the slot).  The last block of a partly filled 64 rows takes its dY through the
-// converters, which write zeros for the rows past the live ones.
+//   warps 3..18   converters, four warps a block (32 rows x 64 columns each), one team of
+//                 them for every operand slot
+//   warps 19..22  epilogue
+// dY, codes and converted rows have rings of their own, each as long as its way round wants:
+// dY is held from its load (some 2800 cycles under load) to the end of its products, the
+// codes until they are converted, the operand from there to the end of the products.  One
+// commit a block, to both CTAs, says that its products are done.  (With one ring of 5 slots
+// for all three the way round was 4100 cycles without any work, 820 a block; two commits a
+// 32-row block kept the issuing thread busy for 1900 cycles.)  The last block of a partly
+// filled 64 rows takes its dY through the converters, which write zeros for the rows past
+// the live ones.
 struct PairSmem {
   static constexpr int kRows = 64;
-  static constexpr int kYBytes = 128 * kRows * 2;
-  static constexpr int kBBytes = 128 * kRows * 2;
-  static constexpr int kQBytes = 128 * kRows;
-  static constexpr int kSlotBytes = kYBytes + kBBytes;
-  static constexpr int kSlots = 6;
-  static constexpr int kQSlots = 4;
-  static constexpr int kWarps = 3 + 2 * kQSlots + 4;
+  static constexpr int kYBytes = 128 * kRows * 2, kYSlots = 7;
+  static constexpr int kBBytes = 128 * kRows * 2, kBSlots = 4;
+  static constexpr int kQBytes = 128 * kRows, kQSlots = 5;
+  static constexpr int kDone = 8;                            // barriers of finished blocks
+  static constexpr int kTeamW = 4;                           // warps of a team
+  static constexpr int kWarps = 3 + kBSlots * kTeamW + 4;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kChain = kChainRows / kRows;
-  static constexpr int kBytes = kSlots * kSlotBytes + kQSlots * kQBytes + 1024 /*align*/;
-  static_assert(kBytes <= 226 * 1024, "ckpt8_dw pair: shared memory");
+  static constexpr int kBytes = kYSlots * kYBytes + kBSlots * kBBytes + kQSlots * kQBytes + 1024 /*align*/;
+  static_assert(kBytes <= 226 * 1024 && kDone >= kYSlots && kQSlots > kBSlots, "ckpt8_dw pair: shared memory");
 };
 
 __global__ void __launch_bounds__(PairSmem::kThreads, 1)
@@ -347,10 +346,11 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
                          Ckpt8DwArgs a, DwPlan plan) {
   GB_PDL_ENTRY();
   using S = PairSmem;
-  constexpr int kSlots = S::kSlots, kQSlots = S::kQSlots, kRows = S::kRows, kChain = S::kChain;
+  constexpr int kYSlots = S::kYSlots, kBSlots = S::kBSlots, kQSlots = S::kQSlots, kDone = S::kDone;
+  constexpr int kRows = S::kRows, kChain = S::kChain;
   constexpr int NT = 256;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t y_full[kSlots], done_bar[kSlots], b_full[kSlots], q_full[kQSlots], q_empty[kQSlots], acc_full[2],
+  __shared__ uint64_t y_full[kYSlots], b_full[kBSlots], q_full[kQSlots], q_empty[kQSlots], done_bar[kDone], acc_full[2],
       acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -362,26 +362,27 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
   const int tile = pair % (plan.m_tiles * plan.n_tiles), split = pair / (plan.m_tiles * plan.n_tiles);
   if (split >= sh.splits) return;  // both CTAs of the pair
   const int m0 = (tile / plan.n_tiles) * 256 + rank * 128, n0 = (tile % plan.n_tiles) * NT + rank * 128;
-  const int kb0 = split * sh.per, nkb = max(0, min(kb_total, kb0 + sh.per) - kb0);
-  // local number of the partly filled block (-1: none here)
-  const int tail = n % kRows != 0 && kb0 + nkb == kb_total ? nkb - 1 : -1;
+  // the splits take the blocks in turn, so that the whole device reads one stretch of rows
+  const int nkb = kb_total > split ? (kb_total - split + sh.splits - 1) / sh.splits : 0;
+  auto row0 = [&](int i) { return (split + i * sh.splits) * kRows; };
+  // number of the partly filled block (-1: none here)
+  const int tail = n % kRows != 0 && nkb > 0 && row0(nkb - 1) + kRows > n ? nkb - 1 : -1;
   float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * NT);
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_area = smem + kSlots * S::kSlotBytes;
+  uint8_t* b_area = smem + kYSlots * S::kYBytes;
+  uint8_t* q_area = b_area + kBSlots * S::kBBytes;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&y_full[s], 1);
-      mbar_init(&done_bar[s], 1);
-      mbar_init(&b_full[s], 4);  // the block's two converters in either CTA
-    }
+    for (int s = 0; s < kYSlots; ++s) mbar_init(&y_full[s], 1);
+    for (int s = 0; s < kBSlots; ++s) mbar_init(&b_full[s], 2 * S::kTeamW);  // the block's team in either CTA
     for (int s = 0; s < kQSlots; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 2);  // the block's two converters
+      mbar_init(&q_empty[s], S::kTeamW);
     }
+    for (int s = 0; s < kDone; ++s) mbar_init(&done_bar[s], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 8);  // four warps in either CTA
@@ -396,141 +397,154 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
 
+  // waits until the products of the pair's block j are done (j in order for every caller,
+  // or after a later block: a wait by parity must not begin two phases early)
+  auto products_done = [&](int j) { return mbar_wait_all(&done_bar[j % kDone], (j / kDone) & 1u, &abort_flag); };
+  // the three issuing warps stay converged; one elected lane issues (elect_one)
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % kSlots;
-        if (i >= kSlots && !mbar_wait(&done_bar[s], ((i / kSlots) & 1u) ^ 1u, &abort_flag)) {
-          set_error(a.err, kErrMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        if (i == tail) {
-          if (rank == 0) mbar_arrive(&y_full[s]);
-          continue;
-        }
-        uint8_t* sy = smem + s * S::kSlotBytes;
-        const int r0 = (kb0 + i) * kRows;
-        if (rank == 0) mbar_expect_tx(&y_full[s], 2 * S::kYBytes);
-        const uint32_t bar = cluster_addr(&y_full[s], 0);
-        tma_load_2d_pair(sy, &tmY, bar, m0, r0);
-        tma_load_2d_pair(sy + 64 * kRows * 2, &tmY, bar, m0 + 64, r0);
-        issued = i + 1;
-      }
-      if (abort_flag && rank == 0) {
-        for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&y_full[i % kSlots], (i / kSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
-          }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = umma_idesc(256, NT, true, true);
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % kSlots;
-        const int chain = i / kChain, ab = chain & 1;
-        const bool first = i % kChain == 0;
-        if ((first && chain >= 2 && !mbar_wait(&acc_empty[ab], ((chain >> 1) - 1) & 1u, &abort_flag)) ||
-            !mbar_wait(&y_full[s], (i / kSlots) & 1u, &abort_flag) ||
-            !mbar_wait(&b_full[s], (i / kSlots) & 1u, &abort_flag)) {
-          set_error(a.err, kErrMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t sy = smem_u32(smem + s * S::kSlotBytes), sb = sy + S::kYBytes;
-#pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk)
-          umma_f16_pair(tmem_base + ab * NT, umma_desc(sy + kk * 2048, 64 * kRows * 2, 1024),
-                        umma_desc(sb + kk * 2048, 64 * kRows * 2, 1024), idesc, (!first || kk > 0) ? 1u : 0u);
-        umma_commit_pair(&done_bar[s]);
-        if (i % kChain == kChain - 1 || i == nkb - 1) umma_commit_pair(&acc_full[ab]);
-      }
-    }
-  } else if (warp == 2) {
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % kQSlots;
-        if (i >= kQSlots && !mbar_wait(&q_empty[s], ((i / kQSlots) & 1u) ^ 1u, &abort_flag)) {
-          set_error(a.err, kErrMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        mbar_expect_tx(&q_full[s], S::kQBytes);
-        tma_load_2d(q_area + s * S::kQBytes, &tmQ, &q_full[s], n0, (kb0 + i) * kRows);
-        issued = i + 1;
-      }
-      if (abort_flag) {
-        for (int i = issued > kQSlots ? issued - kQSlots : 0; i < issued; ++i) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&q_full[i % kQSlots], (i / kQSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
-          }
-        }
-      }
-    }
-  } else if (warp < 3 + 2 * kQSlots) {
-    // A pair of warps keeps to one slot of the codes' ring and takes its blocks in order, so
-    // its wait by parity never begins two phases early; the same holds for the wait on
-    // done_bar, since block i - kQSlots was converted after block i - kQSlots - kSlots's products.
-    const int qs = (warp - 3) >> 1, k = ((warp - 3) & 1) * 32 + lane;  // code slot, row of the block
-    const uint8_t* row = q_area + qs * S::kQBytes + k * 128;
-    uint32_t byte[kAhead][4];
-    auto fetch = [&](int i, uint32_t (&to)[4]) {
-      const int r = (kb0 + i) * kRows + k;
-      const uint8_t* e = a.q8.e + static_cast<int64_t>(r) * a.q8.lde + n0 / 32;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) to[u] = (i < nkb && r < n && n0 / 32 + u < a.groups) ? __ldg(e + u) : 0u;
-    };
-#pragma unroll
-    for (int p = 0; p < kAhead; ++p) fetch(qs + kQSlots * p, byte[p]);
-    for (int i = qs; i < nkb; i += kQSlots) {
-      const int r0 = (kb0 + i) * kRows, s = i % kSlots;
-      uint8_t* sy = smem + s * S::kSlotBytes;
-      uint8_t* sb = sy + S::kYBytes;
-      bool ok = mbar_wait(&q_full[qs], (i / kQSlots) & 1u, &abort_flag);
-      if (ok && i >= kSlots) ok = mbar_wait(&done_bar[s], (i / kSlots - 1) & 1u, &abort_flag);
-      if (!ok) {
+    int issued = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % kYSlots;
+      if (i >= kYSlots && !products_done(i - kYSlots)) {
         if (lane == 0) set_error(a.err, kErrMmaTimeout);
         abort_flag = 1;
         break;
       }
+      uint8_t* sy = smem + s * S::kYBytes;
+      const int r0 = row0(i);
+      if (elect_one()) {
+        if (i == tail) {
+          if (rank == 0) mbar_arrive(&y_full[s]);
+        } else {
+          if (rank == 0) mbar_expect_tx(&y_full[s], 2 * S::kYBytes);
+          const uint32_t bar = cluster_addr(&y_full[s], 0);
+          tma_load_2d_pair(sy, &tmY, bar, m0, r0);
+          tma_load_2d_pair(sy + 64 * kRows * 2, &tmY, bar, m0 + 64, r0);
+        }
+      }
+      __syncwarp();
+      if (i != tail) issued = i + 1;
+    }
+    if (abort_flag && rank == 0) {
+      for (int i = issued > kYSlots ? issued - kYSlots : 0; i < issued; ++i) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&y_full[i % kYSlots], (i / kYSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = umma_idesc(256, NT, true, true);
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % kYSlots, b = i % kBSlots;
+        const int chain = i / kChain, ab = chain & 1;
+        const bool first = i % kChain == 0;
+        if ((first && chain >= 2 && !mbar_wait_all(&acc_empty[ab], ((chain >> 1) - 1) & 1u, &abort_flag)) ||
+            !mbar_wait_all(&y_full[s], (i / kYSlots) & 1u, &abort_flag) ||
+            !mbar_wait_all(&b_full[b], (i / kBSlots) & 1u, &abort_flag)) {
+          if (lane == 0) set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sy = smem_u32(smem + s * S::kYBytes), sb = smem_u32(b_area + b * S::kBBytes);
+        if (elect_one()) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+          for (int kk = 0; kk < kRows / 16; ++kk)
+            umma_f16_pair(tmem_base + ab * NT, umma_desc(sy + kk * 2048, 64 * kRows * 2, 1024),
+                          umma_desc(sb + kk * 2048, 64 * kRows * 2, 1024), idesc, (!first || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&done_bar[i % kDone]);
+          if (i % kChain == kChain - 1 || i == nkb - 1) umma_commit_pair(&acc_full[ab]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 2) {
+    int issued = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % kQSlots;
+      if (i >= kQSlots && !mbar_wait_all(&q_empty[s], ((i / kQSlots) & 1u) ^ 1u, &abort_flag)) {
+        if (lane == 0) set_error(a.err, kErrMmaTimeout);
+        abort_flag = 1;
+        break;
+      }
+      if (elect_one()) {
+        mbar_expect_tx(&q_full[s], S::kQBytes);
+        tma_load_2d(q_area + s * S::kQBytes, &tmQ, &q_full[s], n0, row0(i));
+      }
+      __syncwarp();
+      issued = i + 1;
+    }
+    if (abort_flag) {
+      for (int i = issued > kQSlots ? issued - kQSlots : 0; i < issued; ++i) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&q_full[i % kQSlots], (i / kQSlots) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
+        }
+      }
+    }
+  } else if (warp < 3 + kBSlots * S::kTeamW) {
+    // a team keeps to one operand slot; warp w of it converts rows 32 (w & 1) + lane, columns
+    // 64 (w >> 1) .. + 63: two groups, one 64-column box of the operand
+    const int b = (warp - 3) / S::kTeamW, w = (warp - 3) % S::kTeamW;
+    const int k = (w & 1) * 32 + lane, box = w >> 1;
+    uint8_t* out = b_area + b * S::kBBytes + box * (64 * kRows * 2) + k * 128;
+    const uint32_t full = cluster_addr(&b_full[b], 0);
+    const int g0 = n0 / 32 + 2 * box;
+    uint32_t byte[kAhead][2];
+    auto fetch = [&](int i, uint32_t (&to)[2]) {
+      const int r = row0(i) + k;
+      const uint8_t* e = a.q8.e + static_cast<int64_t>(r) * a.q8.lde + g0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) to[u] = (i < nkb && r < n && g0 + u < a.groups) ? __ldg(e + u) : 0u;
+    };
+#pragma unroll
+    for (int p = 0; p < kAhead; ++p) fetch(b + kBSlots * p, byte[p]);
+    for (int i = b; i < nkb; i += kBSlots) {
+      const int r0 = row0(i), qs = i % kQSlots;
+      // the products of block i - kBSlots are done, so block i - kQSlots was converted and
+      // its codes had come: the next wait begins in their slot's next phase
+      if ((i >= kBSlots && !products_done(i - kBSlots)) ||
+          !mbar_wait_all(&q_full[qs], (i / kQSlots) & 1u, &abort_flag)) {
+        if (lane == 0) set_error(a.err, kErrMmaTimeout);
+        abort_flag = 1;
+        break;
+      }
+      const uint8_t* row = q_area + qs * S::kQBytes + k * 128;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
         const __nv_bfloat162 scale = group8_scale_bf16(byte[0][u]);
-        uint8_t* out = sb + (u >> 1) * (64 * kRows * 2) + k * 128;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint4 c = *reinterpret_cast<const uint4*>(row + (((u * 2 + h) ^ (k & 7)) << 4));
+          const uint4 c = *reinterpret_cast<const uint4*>(row + (((box * 4 + u * 2 + h) ^ (k & 7)) << 4));
           uint4 v0 = values8_bf16(c.x, c.y, scale), v1 = values8_bf16(c.z, c.w, scale);
           if (r0 + k >= n) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);
-          *reinterpret_cast<uint4*>(out + ((((u & 1) * 4 + h * 2) ^ (k & 7)) << 4)) = v0;
-          *reinterpret_cast<uint4*>(out + ((((u & 1) * 4 + h * 2 + 1) ^ (k & 7)) << 4)) = v1;
+          *reinterpret_cast<uint4*>(out + (((u * 4 + h * 2) ^ (k & 7)) << 4)) = v0;
+          *reinterpret_cast<uint4*>(out + (((u * 4 + h * 2 + 1) ^ (k & 7)) << 4)) = v1;
         }
       }
       if (i == tail) {
-        // dY's rows by plain loads (16 pieces of 8 columns), zeros past the live rows
-        const __nv_bfloat16* y = a.dy + static_cast<int64_t>(r0 + k) * a.lddy + m0;
+        // dY's rows by plain loads (a warp eight pieces of 8 columns), zeros past the live
+        // rows.  Its slot: block i - kYSlots is done, as it comes before i - kBSlots
+        const __nv_bfloat16* y = a.dy + static_cast<int64_t>(r0 + k) * a.lddy + m0 + box * 64;
+        uint8_t* sy = smem + (i % kYSlots) * S::kYBytes + box * (64 * kRows * 2) + k * 128;
+        const int cols = a.M - m0 - box * 64;
 #pragma unroll 1
-        for (int p = 0; p < 16; ++p) {
+        for (int p = 0; p < 8; ++p) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (r0 + k < n && m0 + 8 * p < a.M) v = first_columns(*reinterpret_cast<const uint4*>(y + 8 * p), a.M - m0 - 8 * p);
-          *reinterpret_cast<uint4*>(sy + (p >> 3) * (64 * kRows * 2) + k * 128 + (((p & 7) ^ (k & 7)) << 4)) = v;
+          if (r0 + k < n && 8 * p < cols) v = first_columns(*reinterpret_cast<const uint4*>(y + 8 * p), cols - 8 * p);
+          *reinterpret_cast<uint4*>(sy + ((p ^ (k & 7)) << 4)) = v;
         }
       }
 #pragma unroll
       for (int p = 0; p + 1 < kAhead; ++p)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) byte[p][u] = byte[p + 1][u];
-      fetch(i + kQSlots * kAhead, byte[kAhead - 1]);
+        for (int u = 0; u < 2; ++u) byte[p][u] = byte[p + 1][u];
+      fetch(i + kBSlots * kAhead, byte[kAhead - 1]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&q_empty[qs]);
-        mbar_arrive_cluster(cluster_addr(&b_full[s], 0));
+        mbar_arrive_cluster(full);
       }
     }
   } else {
@@ -539,7 +553,7 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
     const int quarter = warp & 3;
     for (int chain = 0; chain * kChain < nkb; ++chain) {
       const int ab = chain & 1;
-      if (!mbar_wait(&acc_full[ab], (chain >> 1) & 1u, &abort_flag)) {
+      if (!mbar_wait_all(&acc_full[ab], (chain >> 1) & 1u, &abort_flag)) {
         if (lane == 0) set_error(a.err, kErrMmaTimeout);
         abort_flag = 1;
         break;

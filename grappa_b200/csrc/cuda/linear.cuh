@@ -129,23 +129,24 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
 
+  // the two issuing warps stay converged; one elected lane issues (elect_one)
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool stop = false;
-      for (int64_t t = first; t < tiles && !stop; t += step) {
-        const int m0 = static_cast<int>(t / n_tiles) * kTileM + rank * BM;
-        const int n0 = static_cast<int>(t % n_tiles) * BN + rank * S::kBRows;
-        for (int kb = 0; kb < kbs; ++kb, ++it) {
-          const int s = static_cast<int>(it % kStages);
-          if (it >= static_cast<uint32_t>(kStages) &&
-              !mbar_wait(&empty_bar[s], ((it / kStages) & 1u) ^ 1u, &abort_flag)) {
-            set_error(a.err, kErrMmaTimeout);
-            abort_flag = 1;
-            stop = true;
-            break;
-          }
-          uint8_t* sa = smem + s * S::kStageBytes;
+    uint32_t it = 0;
+    bool stop = false;
+    for (int64_t t = first; t < tiles && !stop; t += step) {
+      const int m0 = static_cast<int>(t / n_tiles) * kTileM + rank * BM;
+      const int n0 = static_cast<int>(t % n_tiles) * BN + rank * S::kBRows;
+      for (int kb = 0; kb < kbs; ++kb, ++it) {
+        const int s = static_cast<int>(it % kStages);
+        if (it >= static_cast<uint32_t>(kStages) &&
+            !mbar_wait_all(&empty_bar[s], ((it / kStages) & 1u) ^ 1u, &abort_flag)) {
+          if (lane == 0) set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          stop = true;
+          break;
+        }
+        uint8_t* sa = smem + s * S::kStageBytes;
+        if (elect_one()) {
           if constexpr (CG == 2) {
             // both CTAs' loads complete on the issuing CTA's barrier
             if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * S::kStageBytes);
@@ -158,37 +159,36 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
             tma_load_2d(sa + S::kABytes, &tmW, &full_bar[s], kb * BK, n0);
           }
         }
+        __syncwarp();
       }
-      // on abort, wait (bounded) for the loads still in flight (of both CTAs)
-      if (abort_flag && rank == 0) {
-        for (uint32_t i = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u; i < it; ++i) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&full_bar[i % kStages], (i / kStages) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
-          }
+    }
+    // on abort, wait (bounded) for the loads still in flight (of both CTAs)
+    if (abort_flag && rank == 0) {
+      for (uint32_t i = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u; i < it; ++i) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&full_bar[i % kStages], (i / kStages) & 1u) && globaltimer_ns() - t0 < kWaitNs) {
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = umma_idesc(kTileM, BN, false, false);
       uint32_t it = 0;
       int lt = 0;
       bool stop = false;
       for (int64_t t = first; t < tiles && !stop; t += step, ++lt) {
         const int b = lt & 1;
-        if (lt >= 2) {
-          const uint32_t parity = ((lt >> 1) - 1) & 1u;
-          if (!mbar_wait(&acc_empty[b], parity, &abort_flag)) {
-            set_error(a.err, kErrMmaTimeout);
-            abort_flag = 1;
-            break;
-          }
+        if (lt >= 2 && !mbar_wait_all(&acc_empty[b], ((lt >> 1) - 1) & 1u, &abort_flag)) {
+          if (lane == 0) set_error(a.err, kErrMmaTimeout);
+          abort_flag = 1;
+          break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem_base + static_cast<uint32_t>(b * BN);
         for (int kb = 0; kb < kbs; ++kb, ++it) {
           const int s = static_cast<int>(it % kStages);
-          if (!mbar_wait(&full_bar[s], (it / kStages) & 1u, &abort_flag)) {
-            set_error(a.err, kErrMmaTimeout);
+          if (!mbar_wait_all(&full_bar[s], (it / kStages) & 1u, &abort_flag)) {
+            if (lane == 0) set_error(a.err, kErrMmaTimeout);
             abort_flag = 1;
             stop = true;
             break;
@@ -196,15 +196,18 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t sa = smem_u32(smem + s * S::kStageBytes);
           const uint32_t sb = sa + S::kABytes;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            const uint32_t d = tmem_base + static_cast<uint32_t>(b * BN), acc = (kb > 0 || kk > 0) ? 1u : 0u;
-            const uint64_t da = umma_desc(sa + kk * 32, 16, 1024), db = umma_desc(sb + kk * 32, 16, 1024);
-            CG == 2 ? umma_f16_pair(d, da, db, idesc, acc) : umma_f16(d, da, db, idesc, acc);
+            for (int kk = 0; kk < BK / 16; ++kk) {
+              const uint32_t acc = (kb > 0 || kk > 0) ? 1u : 0u;
+              const uint64_t da = umma_desc(sa + kk * 32, 16, 1024), db = umma_desc(sb + kk * 32, 16, 1024);
+              CG == 2 ? umma_f16_pair(d, da, db, idesc, acc) : umma_f16(d, da, db, idesc, acc);
+            }
+            CG == 2 ? umma_commit_pair(&empty_bar[s]) : umma_commit(&empty_bar[s]);
+            if (kb == kbs - 1) CG == 2 ? umma_commit_pair(&acc_full[b]) : umma_commit(&acc_full[b]);
           }
-          CG == 2 ? umma_commit_pair(&empty_bar[s]) : umma_commit(&empty_bar[s]);
+          __syncwarp();
         }
-        if (!stop) CG == 2 ? umma_commit_pair(&acc_full[b]) : umma_commit(&acc_full[b]);
       }
     }
   } else {
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
       const bool live = m < M;
       const bool slab_full = m0 + 32 <= M;  // rows past M are not written: no TMA store of such a slab
       const int ab = lt & 1;
-      if (!mbar_wait(&acc_full[ab], (lt >> 1) & 1u, &abort_flag)) {
+      if (!mbar_wait_all(&acc_full[ab], (lt >> 1) & 1u, &abort_flag)) {
         if (lane == 0) set_error(a.err, kErrMmaTimeout);
         abort_flag = 1;
         break;
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
         if (h == 0 || t + step < tiles) ++asked;
         __syncwarp();
         if (has_res) {
-          if (!mbar_wait(&res_full[w][h], lt & 1u, &abort_flag)) {
+          if (!mbar_wait_all(&res_full[w][h], lt & 1u, &abort_flag)) {
             if (lane == 0) set_error(a.err, kErrMmaTimeout);
             abort_flag = 1;
             stop = true;
