@@ -140,7 +140,7 @@ c10::Device on_device(std::initializer_list<const Tensor*> ts, std::initializer_
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 Tensor work_area(int64_t floats, c10::Device dev) {
-  return at::empty({std::max<int64_t>(floats, 4)}, at::TensorOptions().dtype(at::kFloat).device(dev));
+  return floats > 0 ? at::empty({floats}, at::TensorOptions().dtype(at::kFloat).device(dev)) : Tensor();
 }
 
 void dropout_args(double p, const OptT& counters, float* out_p, const int64_t** out_c) {
@@ -251,7 +251,7 @@ void rmsnorm_bwd(Tensor dy, OptT x, Tensor rstd, Tensor gamma, int64_t dim, OptT
   const auto dev = on_device({&dy, &rstd, &gamma, &dx, &dgamma}, {&x, &n_dev, &dres, &n_res_dev, &q, &q_exp});
   c10::cuda::CUDAGuard g(dev);
   const Tensor work = work_area(d::rmsnorm_bwd_work_floats(a.dim, a.cap, sms()), dev);
-  a.work = work.data_ptr<float>();
+  a.work = work.defined() ? work.data_ptr<float>() : nullptr;
   d::launch_rmsnorm_bwd(a, sms(), stream());
 }
 
@@ -356,7 +356,7 @@ void linear_act_bwd(Tensor dout, int64_t dim, OptT n_dev, int64_t cap, int64_t a
   Tensor work;
   if (a.dbias) {
     work = work_area(d::linear_act_bwd_work_floats(a.dim, a.cap, sms()), dev);
-    a.work = work.data_ptr<float>();
+    a.work = work.defined() ? work.data_ptr<float>() : nullptr;
   }
   d::launch_linear_act_bwd(a, sms(), stream());
 }
@@ -424,7 +424,7 @@ void ckpt8_dw(Tensor dy, Tensor q, Tensor q_exp, OptT n_dev, int64_t cap, Tensor
   const auto dev = on_device({&dy, &q, &q_exp, &gw, &err}, {&n_dev});
   c10::cuda::CUDAGuard g(dev);
   const Tensor work = work_area(d::ckpt8_dw_work_floats(a.M, a.N, a.cap, sms()), dev);
-  a.work = work.data_ptr<float>();
+  a.work = work.defined() ? work.data_ptr<float>() : nullptr;
   d::launch_ckpt8_dw(a, sms(), stream());
 }
 

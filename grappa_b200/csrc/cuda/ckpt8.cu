@@ -230,41 +230,52 @@ __global__ void __launch_bounds__(kThreads, 4) linear_act_bwd_kernel(LinearActBw
 #pragma unroll
   for (int j = 0; j < 8; ++j) parts[team][t * 8 + j] = acc[j];
   __syncthreads();
-  const int col = blockIdx.y * 256 + threadIdx.x;
-  if (threadIdx.x < LPR * 8 && col < a.dim) {
-    float s = 0.f;
+  const int col0 = blockIdx.y * 256;
+  float s = 0.f;
+  if (threadIdx.x < LPR * 8) {
 #pragma unroll 8
     for (int p = 0; p < kTeams; ++p) s += parts[p][threadIdx.x];
-    a.work[static_cast<int64_t>(blockIdx.x) * a.dim + col] = s;
+  }
+  if (a.cluster) {
+    // the slice's CTAs are one cluster, which finishes the sums
+    __shared__ float cols[LPR * 8];
+    if (threadIdx.x < LPR * 8) cols[threadIdx.x] = s;
+    cluster_column_sums(cols, min(LPR * 8, a.dim - col0), a.dbias + col0, a.accumulate);
+  } else if (threadIdx.x < LPR * 8 && col0 + static_cast<int>(threadIdx.x) < a.dim) {
+    a.work[static_cast<int64_t>(blockIdx.x) * a.dim + col0 + threadIdx.x] = s;
   }
 }
 
 constexpr int kCtasPerSm = 4;
 
-int act_bwd_grid(int dim, int cap, int num_sms) {
+int64_t act_bwd_passes(int dim, int cap) {
   const int lpr = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
+  return ceil_div(std::max(cap, 1), kThreads / lpr * kRows);
+}
+int act_bwd_grid(int dim, int cap, int num_sms) {
   const int64_t slices = ceil_div(dim, 256);
-  const int64_t want = ceil_div(std::max(cap, 1), kThreads / lpr * kRows);
   return static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(want, std::max<int64_t>(1, static_cast<int64_t>(num_sms) * kCtasPerSm / slices))));
+      1, std::min<int64_t>(act_bwd_passes(dim, cap), std::max<int64_t>(1, static_cast<int64_t>(num_sms) * kCtasPerSm / slices))));
 }
 
 template <int LPR>
 void act_bwd_t(const LinearActBwdArgs& a, dim3 grid, cudaStream_t stream) {
   auto kern = a.dout_f32 ? (a.q8.q ? linear_act_bwd_kernel<LPR, true, true> : linear_act_bwd_kernel<LPR, true, false>)
                          : (a.q8.q ? linear_act_bwd_kernel<LPR, false, true> : linear_act_bwd_kernel<LPR, false, false>);
-  launch_k(kern, grid, dim3(kThreads), 0, stream, a);
+  launch_cluster_k(kern, grid, dim3(kThreads), a.cluster ? grid.x : 1u, 0, stream, a);
   GB_LAUNCH_CHECK();
 }
 
 }  // namespace
 
 int64_t linear_act_bwd_work_floats(int dim, int cap, int num_sms) {
-  return static_cast<int64_t>(dim) * act_bwd_grid(dim, cap, num_sms);
+  return act_bwd_passes(dim, cap) <= kClusterPasses ? 0 : static_cast<int64_t>(dim) * act_bwd_grid(dim, cap, num_sms);
 }
 
-void launch_linear_act_bwd(const LinearActBwdArgs& a, int num_sms, cudaStream_t stream) {
-  const int gx = act_bwd_grid(a.dim, a.cap, num_sms);
+void launch_linear_act_bwd(LinearActBwdArgs a, int num_sms, cudaStream_t stream) {
+  int gx = act_bwd_grid(a.dim, a.cap, num_sms);
+  a.cluster = a.dbias && act_bwd_passes(a.dim, a.cap) <= kClusterPasses;
+  if (a.cluster) gx = std::min(gx, 8);
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(ceil_div(a.dim, 256)));
   if (a.dim <= 32)
     act_bwd_t<4>(a, grid, stream);
@@ -274,7 +285,7 @@ void launch_linear_act_bwd(const LinearActBwdArgs& a, int num_sms, cudaStream_t 
     act_bwd_t<16>(a, grid, stream);
   else
     act_bwd_t<32>(a, grid, stream);
-  if (a.dbias) launch_sum_parts(a.work, gx, a.dim, a.dim, a.dbias, a.accumulate, stream);
+  if (a.dbias && !a.cluster) launch_sum_parts(a.work, gx, a.dim, a.dim, a.dbias, a.accumulate, stream);
 }
 
 void launch_ckpt8_store(const Ckpt8Args& a, cudaStream_t stream) {

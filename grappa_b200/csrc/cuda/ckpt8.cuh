@@ -145,5 +145,24 @@ __device__ __forceinline__ int live_rows(const int32_t* n_ptr, int cap) {
 void launch_sum_parts(const float* part, int parts, int64_t ld, int cols, float* out, bool accumulate,
                       cudaStream_t stream);
 
+// Up to this many passes of a row kernel's CTA are left to one cluster (four rounds of it).
+constexpr int kClusterPasses = 32;
+
+// out[c] (+)= sum over the cluster's CTAs, in order, of cols[c] in their shared memory; the CTAs
+// share the columns.  Called by all threads of all CTAs; cols was written by this CTA.
+__device__ __forceinline__ void cluster_column_sums(const float* cols, int n, float* out, bool accumulate) {
+  uint32_t ctas;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+  __syncthreads();
+  cluster_sync();
+  const int first = static_cast<int>(cluster_rank() * blockDim.x + threadIdx.x);
+  for (int c = first; c < n; c += static_cast<int>(ctas * blockDim.x)) {
+    float s = 0.f;
+    for (uint32_t r = 0; r < ctas; ++r) s += ld_cluster(cluster_addr(cols + c, r));
+    out[c] = (accumulate ? out[c] : 0.f) + s;
+  }
+  cluster_sync();  // the others may still read this CTA's sums
+}
+
 }  // namespace dev
 }  // namespace grappa

@@ -35,7 +35,9 @@ constexpr int kTeam = 4;
 constexpr int kTeams = kConv / kTeam;
 constexpr int kThreads = 64 + 32 * kConv;
 constexpr int kAhead = 2;
-constexpr int kChainRows = 4096;
+constexpr int kClusterKb = 48;     // blocks a split at most where the splits are a cluster
+static_assert(kClusterKb * BK <= 2048, "one chain");
+constexpr int kChainRows = 2048;
 constexpr int kChainKb = kChainRows / BK;
 
 template <int MT, int NT>
@@ -71,29 +73,35 @@ struct DwPlan {
   int rows;              // of a block
   int splits, min_kb;    // CTAs (pairs) a tile at most, blocks each at least
   bool pair = false;     // by CTA pairs (mt = 2, nt = 256)
+  bool cluster = false;  // a tile's splits are one cluster that sums its partial tiles itself
   bool y_blocks = false, q_blocks = false;  // operands of whole column blocks (64 bf16, 128 codes)
 };
+
+// Four sums at place `at` of a tile in the partial tiles' order, into gW.
+__device__ __forceinline__ void add_quad(const Ckpt8DwArgs& a, const DwPlan& plan, int tile, int at, float4 s) {
+  // at = ((c / 32) * 4 + quarter) * 1024 + j * 128 + lane * 4
+  const int lane = (at / 4) % 32, j = (at / 128) % 8, quarter = (at / 1024) % 4, c32 = at / 4096;
+  const int col_t = c32 * 32 + j * 4;  // column over the MT accumulators
+  const int m = (tile / plan.n_tiles) * 128 * plan.mt + (col_t / plan.nt) * 128 + quarter * 32 + lane;
+  const int nn = (tile % plan.n_tiles) * plan.nt + col_t % plan.nt;
+  if (m >= a.M || nn >= a.N) return;
+  float* g = a.gw + static_cast<int64_t>(m) * a.ldg + nn;
+  const float o[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (nn + q < a.N) g[q] = (a.accumulate ? g[q] : 0.f) + o[q];
+}
 
 template <int MT, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     ckpt8_dw_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmQ, Ckpt8DwArgs a,
                     DwPlan plan) {
-  GB_PDL_ENTRY();
   using S = DSmem<MT, NT>;
   constexpr int kSlots = S::kSlots;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[kSlots], empty_bar[kSlots], b_full[kTeams], b_empty[kTeams], acc_full, acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-
-  const int n = live_rows(a.n_ptr, a.cap);
-  const int kb_total = (n + BK - 1) / BK;
-  const Shares sh = shares(kb_total, plan.splits, plan.min_kb);
-  const int tile = blockIdx.x % (plan.m_tiles * plan.n_tiles), split = blockIdx.x / (plan.m_tiles * plan.n_tiles);
-  if (split >= sh.splits) return;
-  const int m0 = (tile / plan.n_tiles) * (128 * MT), n0 = (tile % plan.n_tiles) * NT;
-  const int kb0 = split * sh.per, kb1 = min(kb_total, kb0 + sh.per);
-  float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * MT * NT);
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* b_area = smem + kSlots * S::kSlotBytes;
@@ -113,12 +121,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&acc_empty, kConv);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&tmY);
+    prefetch_map(&tmQ);
   }
   if (warp == 1) tmem_alloc(&tmem_slot, S::kTmemCols);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
+  // all of this may run while the kernel before is ending; its results are read from here on
+  GB_PDL_ENTRY();
+  const int n = live_rows(a.n_ptr, a.cap);
+  const int kb_total = (n + BK - 1) / BK;
+  const Shares sh = shares(kb_total, plan.splits, plan.min_kb);
+  // the splits of a tile are a cluster (plan.cluster), or tiles apart
+  const int tiles = plan.m_tiles * plan.n_tiles;
+  const int tile = plan.cluster ? blockIdx.x / plan.splits : blockIdx.x % tiles;
+  const int split = plan.cluster ? blockIdx.x % plan.splits : blockIdx.x / tiles;
+  const int m0 = (tile / plan.n_tiles) * (128 * MT), n0 = (tile % plan.n_tiles) * NT;
+  const int kb0 = split * sh.per, kb1 = split < sh.splits ? min(kb_total, kb0 + sh.per) : kb0;
+  float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * MT * NT);
   const int nkb = max(0, kb1 - kb0);
 
   // the two issuing warps stay converged; one elected lane issues (elect_one)
@@ -285,7 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = share * (MT * NT / 4); c < (share + 1) * (MT * NT / 4); c += 32) {
         float v[32];
         tmem_ld32(tmem_base + static_cast<uint32_t>(c) + (static_cast<uint32_t>(quarter * 32) << 16), v);
-        float* p = part + (static_cast<int64_t>(c / 32) * 4 + quarter) * 1024 + lane * 4;
+        // (a cluster's CTA keeps it in its own shared memory, where the ring was: its only chain
+        // is over, so every load and product of the ring is)
+        float* p = (plan.cluster ? reinterpret_cast<float*>(smem) : part) +
+                   (static_cast<int64_t>(c / 32) * 4 + quarter) * 1024 + lane * 4;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (chunk == 0)
@@ -300,6 +325,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
+  if (plan.cluster) {
+    // gW (+)= the cluster's partial tiles, in order, each CTA a share of the tile
+    cluster_sync();
+    constexpr int kQuads = 128 * MT * NT / 4;
+    const int splits = kb_total > 0 ? sh.splits : 0;
+    for (int x = split * kThreads + static_cast<int>(threadIdx.x); x < kQuads; x += plan.splits * kThreads) {
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < splits) v[r] = ld_cluster4(cluster_addr(smem + x * 16, static_cast<uint32_t>(r)));
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s.x += v[r].x, s.y += v[r].y, s.z += v[r].z, s.w += v[r].w;
+      add_quad(a, plan, tile, x * 4, s);
+    }
+    cluster_sync();  // the others may still read this CTA's tile
+  }
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_dealloc(tmem_base, S::kTmemCols);
@@ -312,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // SM that halves the operand bytes that the tensor core reads from shared memory (which
 // bound the single CTA: 96 KB of traffic a 32-row block against 512 cycles of products),
 // and the accumulator takes half of TMEM, so there are two: four warps of their own empty
-// one while the products of the next 4096 rows fill the other.
+// one while the products of the next 2048 rows fill the other.
 //   warp 0        TMA producer of dY: 128 columns a CTA, on CTA 0's barrier
 //   warp 1        (CTA 0) issues the products
 //   warp 2        TMA producer of the codes, on the CTA's own barriers
@@ -344,7 +388,6 @@ struct PairSmem {
 __global__ void __launch_bounds__(PairSmem::kThreads, 1)
     ckpt8_dw_pair_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmQ,
                          Ckpt8DwArgs a, DwPlan plan) {
-  GB_PDL_ENTRY();
   using S = PairSmem;
   constexpr int kYSlots = S::kYSlots, kBSlots = S::kBSlots, kQSlots = S::kQSlots, kDone = S::kDone;
   constexpr int kRows = S::kRows, kChain = S::kChain;
@@ -354,20 +397,6 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
       acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-
-  const int n = live_rows(a.n_ptr, a.cap);
-  const int kb_total = (n + kRows - 1) / kRows;
-  const Shares sh = shares(kb_total, plan.splits, plan.min_kb);
-  const int pair = blockIdx.x >> 1, rank = static_cast<int>(cluster_rank());
-  const int tile = pair % (plan.m_tiles * plan.n_tiles), split = pair / (plan.m_tiles * plan.n_tiles);
-  if (split >= sh.splits) return;  // both CTAs of the pair
-  const int m0 = (tile / plan.n_tiles) * 256 + rank * 128, n0 = (tile % plan.n_tiles) * NT + rank * 128;
-  // the splits take the blocks in turn, so that the whole device reads one stretch of rows
-  const int nkb = kb_total > split ? (kb_total - split + sh.splits - 1) / sh.splits : 0;
-  auto row0 = [&](int i) { return (split + i * sh.splits) * kRows; };
-  // number of the partly filled block (-1: none here)
-  const int tail = n % kRows != 0 && nkb > 0 && row0(nkb - 1) + kRows > n ? nkb - 1 : -1;
-  float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * NT);
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* b_area = smem + kYSlots * S::kYBytes;
@@ -389,6 +418,8 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&tmY);
+    prefetch_map(&tmQ);
   }
   if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * NT);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -397,6 +428,20 @@ __global__ void __launch_bounds__(PairSmem::kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
 
+  // all of this may run while the kernel before is ending; its results are read from here on
+  GB_PDL_ENTRY();
+  const int n = live_rows(a.n_ptr, a.cap);
+  const int kb_total = (n + kRows - 1) / kRows;
+  const Shares sh = shares(kb_total, plan.splits, plan.min_kb);
+  const int pair = blockIdx.x >> 1, rank = static_cast<int>(cluster_rank());
+  const int tile = pair % (plan.m_tiles * plan.n_tiles), split = pair / (plan.m_tiles * plan.n_tiles);
+  const int m0 = (tile / plan.n_tiles) * 256 + rank * 128, n0 = (tile % plan.n_tiles) * NT + rank * 128;
+  // the splits take the blocks in turn, so that the whole device reads one stretch of rows
+  const int nkb = split < sh.splits && kb_total > split ? (kb_total - split + sh.splits - 1) / sh.splits : 0;
+  auto row0 = [&](int i) { return (split + i * sh.splits) * kRows; };
+  // number of the partly filled block (-1: none here)
+  const int tail = n % kRows != 0 && nkb > 0 && row0(nkb - 1) + kRows > n ? nkb - 1 : -1;
+  float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * NT);
   // waits until the products of the pair's block j are done (j in order for every caller,
   // or after a later block: a wait by parity must not begin two phases early)
   auto products_done = [&](int j) { return mbar_wait_all(&done_bar[j % kDone], (j / kDone) & 1u, &abort_flag); };
@@ -622,23 +667,15 @@ __global__ void __launch_bounds__(256) ckpt8_dw_sum_kernel(Ckpt8DwArgs a, DwPlan
     s.z += v.z;
     s.w += v.w;
   }
-  // at = ((c / 32) * 4 + quarter) * 1024 + j * 128 + lane * 4
-  const int lane = (at / 4) % 32, j = (at / 128) % 8, quarter = (at / 1024) % 4, c32 = at / 4096;
-  const int col_t = c32 * 32 + j * 4;  // column over the MT accumulators
-  const int m = (tile / plan.n_tiles) * 128 * plan.mt + (col_t / plan.nt) * 128 + quarter * 32 + lane;
-  const int nn = (tile % plan.n_tiles) * plan.nt + col_t % plan.nt;
-  if (m >= a.M || nn >= a.N) return;
-  float* g = a.gw + static_cast<int64_t>(m) * a.ldg + nn;
-  const float o[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    if (nn + q < a.N) g[q] = (a.accumulate ? g[q] : 0.f) + o[q];
+  add_quad(a, plan, tile, at, s);
 }
 
 // Tile and shares for M x N over cap rows on num_sms SMs.  The large tile (256 x 256) reads
 // each operand least often and converts each code once per 256 columns of dY; it needs
 // enough rows for every SM to get some 32 blocks of them.  With fewer rows the small tile
-// spreads the same work over four times as many CTAs.
+// spreads the same work over four times as many CTAs, and few rows are split over the CTAs
+// of one cluster, which sum their partial tiles over distributed shared memory: no second
+// kernel and no work area.
 DwPlan plan_for(int M, int N, int cap, int num_sms) {
   DwPlan p;
   int64_t kb = ceil_div(std::max(cap, 1), BK);
@@ -660,6 +697,12 @@ DwPlan plan_for(int M, int N, int cap, int num_sms) {
     kb = ceil_div(std::max(cap, 1), p.rows);
   }
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  // a split's only chain: its partial tile needs no earlier ones
+  if (p.mt == 1 && p.nt == 128 && kb <= 8 * kClusterKb) {
+    p.cluster = true;
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, kb / p.min_kb)));
+    return p;
+  }
   const int64_t at_once = p.pair ? num_sms / 2 : num_sms;
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(at_once / tiles, kb / p.min_kb)));
   return p;
@@ -685,8 +728,8 @@ void launch_t(const Ckpt8DwArgs& a, DwPlan p, cudaStream_t stream) {
                                     : map_q(a, BK);
   auto kern = ckpt8_dw_kernel<MT, NT>;
   set_smem(reinterpret_cast<const void*>(kern), S::kBytes);
-  launch_k(kern, dim3(static_cast<unsigned>(p.m_tiles * p.n_tiles * p.splits)), dim3(kThreads), S::kBytes, stream, my,
-           mq, a, p);
+  launch_cluster_k(kern, dim3(static_cast<unsigned>(p.m_tiles * p.n_tiles * p.splits)), dim3(kThreads),
+                   p.cluster ? static_cast<unsigned>(p.splits) : 1u, S::kBytes, stream, my, mq, a, p);
   GB_LAUNCH_CHECK();
 }
 
@@ -703,7 +746,7 @@ void launch_pair(const Ckpt8DwArgs& a, DwPlan p, cudaStream_t stream) {
 
 int64_t ckpt8_dw_work_floats(int M, int N, int cap, int num_sms) {
   const DwPlan p = plan_for(M, N, cap, num_sms);
-  return static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits * 128 * p.mt * p.nt;
+  return p.cluster ? 0 : static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits * 128 * p.mt * p.nt;
 }
 
 void launch_ckpt8_dw(const Ckpt8DwArgs& a, int num_sms, cudaStream_t stream) {
@@ -714,6 +757,7 @@ void launch_ckpt8_dw(const Ckpt8DwArgs& a, int num_sms, cudaStream_t stream) {
     launch_t<2, 128>(a, p, stream);
   else
     p.nt == 256 ? launch_t<1, 256>(a, p, stream) : launch_t<1, 128>(a, p, stream);
+  if (p.cluster) return;
   const int64_t threads = static_cast<int64_t>(p.m_tiles) * p.n_tiles * 128 * p.mt * p.nt / 4;
   launch_k(ckpt8_dw_sum_kernel, dim3(static_cast<unsigned>(threads / 64)), dim3(256), 0, stream, a, p);
   GB_LAUNCH_CHECK();

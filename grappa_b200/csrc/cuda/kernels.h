@@ -546,7 +546,8 @@ struct RmsNormBwdArgs {
   int64_t lddx = 0;
   float* dgamma = nullptr;          // [dim]
   bool accumulate = true;
-  float* work = nullptr;            // rmsnorm_bwd_work_floats() floats
+  float* work = nullptr;            // rmsnorm_bwd_work_floats() floats (none: null)
+  bool cluster = false;             // set by the launcher: the grid is one cluster
 };
 int64_t rmsnorm_bwd_work_floats(int dim, int cap, int num_sms);
 void launch_rmsnorm_bwd(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream);
@@ -607,10 +608,11 @@ struct LinearActBwdArgs {
   int64_t lddz = 0;
   float* dbias = nullptr;
   bool accumulate = true;
-  float* work = nullptr;
+  float* work = nullptr;            // linear_act_bwd_work_floats() floats (none: null)
+  bool cluster = false;             // set by the launcher: the grid's x is one cluster
 };
 int64_t linear_act_bwd_work_floats(int dim, int cap, int num_sms);
-void launch_linear_act_bwd(const LinearActBwdArgs& a, int num_sms, cudaStream_t stream);
+void launch_linear_act_bwd(LinearActBwdArgs a, int num_sms, cudaStream_t stream);
 
 struct Ckpt8Args {
   const void* x = nullptr;          // store: the rows; load: unused

@@ -78,7 +78,6 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
     linear_fwd_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                       const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmO,
                       const __grid_constant__ CUtensorMap tmQ, LinearArgs a) {
-  GB_PDL_ENTRY();
   using S = LSmem<BN, CG>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -93,16 +92,6 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
   const int act = ANY ? a.act : ACT;
   const bool has_res = ANY ? a.residual != nullptr : RES;
   const bool has_q8 = ANY ? a.q8.q != nullptr : Q8;
-  const int M = live_rows(a.n_ptr, a.cap);
-  const int kbs = (a.K + BK - 1) / BK;
-  const int n_tiles = (a.N + BN - 1) / BN;
-  // a tile is CG * 128 rows x BN columns; CTA `rank` of the pair has rows rank * 128 .. + 127
-  constexpr int kTileM = BM * CG;
-  const int64_t tiles = static_cast<int64_t>((M + kTileM - 1) / kTileM) * n_tiles;
-  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
-  if (first >= tiles) return;
-  const int rank = CG == 2 ? static_cast<int>(cluster_rank()) : 0;
-
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* out_area = smem + kStages * S::kStageBytes;
   uint8_t* code_area = out_area + S::kOutBytes;
@@ -121,6 +110,10 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&tmA);
+    prefetch_map(&tmW);
+    prefetch_map(&tmO);
+    if (has_res) prefetch_map(&tmR);
   }
   if (warp == 1) CG == 2 ? tmem_alloc_pair(&tmem_slot, S::kTmemCols) : tmem_alloc(&tmem_slot, S::kTmemCols);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -128,6 +121,16 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
   if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers are ready
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
+  // all of this may run while the kernel before is ending; its results are read from here on
+  GB_PDL_ENTRY();
+  const int M = live_rows(a.n_ptr, a.cap);
+  const int kbs = (a.K + BK - 1) / BK;
+  const int n_tiles = (a.N + BN - 1) / BN;
+  // a tile is CG * 128 rows x BN columns; CTA `rank` of the pair has rows rank * 128 .. + 127
+  constexpr int kTileM = BM * CG;
+  const int64_t tiles = static_cast<int64_t>((M + kTileM - 1) / kTileM) * n_tiles;
+  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int rank = CG == 2 ? static_cast<int>(cluster_rank()) : 0;
 
   // the two issuing warps stay converged; one elected lane issues (elect_one)
   if (warp == 0) {
@@ -234,8 +237,8 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
       tma_load_2d(panels + h * 2048, &tmR, &res_full[w][h], static_cast<int>(t % n_tiles) * BN + col0 + h * 32,
                   static_cast<int>(t / n_tiles) * kTileM + rank * BM + quarter * 32);
     };
-    if (has_res && lane == 0) ask(first, 0);
-    int asked = 1, taken = 0;  // residual half panels asked for and arrived
+    if (has_res && lane == 0 && first < tiles) ask(first, 0);
+    int asked = first < tiles ? 1 : 0, taken = 0;  // residual half panels asked for and arrived
     int lt = 0;
     bool stop = false;
     for (int64_t t = first; t < tiles && !stop; t += step, ++lt) {
