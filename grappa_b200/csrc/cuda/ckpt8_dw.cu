@@ -77,15 +77,19 @@ struct DwPlan {
   bool y_blocks = false, q_blocks = false;  // operands of whole column blocks (64 bf16, 128 codes)
 };
 
-// Four sums at place `at` of a tile in the partial tiles' order, into gW.
-__device__ __forceinline__ void add_quad(const Ckpt8DwArgs& a, const DwPlan& plan, int tile, int at, float4 s) {
-  // at = ((c / 32) * 4 + quarter) * 1024 + j * 128 + lane * 4
-  const int lane = (at / 4) % 32, j = (at / 128) % 8, quarter = (at / 1024) % 4, c32 = at / 4096;
-  const int col_t = c32 * 32 + j * 4;  // column over the MT accumulators
-  const int m = (tile / plan.n_tiles) * 128 * plan.mt + (col_t / plan.nt) * 128 + quarter * 32 + lane;
-  const int nn = (tile % plan.n_tiles) * plan.nt + col_t % plan.nt;
+// Four sums into row m, columns nn .. nn + 3 of gW.
+__device__ __forceinline__ void add_quad(const Ckpt8DwArgs& a, int m, int nn, float4 s) {
   if (m >= a.M || nn >= a.N) return;
   float* g = a.gw + static_cast<int64_t>(m) * a.ldg + nn;
+  if (nn + 4 <= a.N && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+    float4* g4 = reinterpret_cast<float4*>(g);
+    if (a.accumulate) {
+      const float4 o = *g4;
+      s.x += o.x, s.y += o.y, s.z += o.z, s.w += o.w;
+    }
+    *g4 = s;
+    return;
+  }
   const float o[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
   for (int q = 0; q < 4; ++q)
@@ -98,6 +102,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     DwPlan plan) {
   using S = DSmem<MT, NT>;
   constexpr int kSlots = S::kSlots;
+  const bool cluster = MT == 1 && NT == 128 && plan.cluster;  // only the small tile's plans set it
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[kSlots], empty_bar[kSlots], b_full[kTeams], b_empty[kTeams], acc_full, acc_empty;
   __shared__ uint32_t tmem_slot;
@@ -136,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Shares sh = shares(kb_total, plan.splits, plan.min_kb);
   // the splits of a tile are a cluster (plan.cluster), or tiles apart
   const int tiles = plan.m_tiles * plan.n_tiles;
-  const int tile = plan.cluster ? blockIdx.x / plan.splits : blockIdx.x % tiles;
-  const int split = plan.cluster ? blockIdx.x % plan.splits : blockIdx.x / tiles;
+  const int tile = cluster ? blockIdx.x / plan.splits : blockIdx.x % tiles;
+  const int split = cluster ? blockIdx.x % plan.splits : blockIdx.x / tiles;
   const int m0 = (tile / plan.n_tiles) * (128 * MT), n0 = (tile % plan.n_tiles) * NT;
   const int kb0 = split * sh.per, kb1 = split < sh.splits ? min(kb_total, kb0 + sh.per) : kb0;
   float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * MT * NT);
@@ -307,10 +312,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = share * (MT * NT / 4); c < (share + 1) * (MT * NT / 4); c += 32) {
         float v[32];
         tmem_ld32(tmem_base + static_cast<uint32_t>(c) + (static_cast<uint32_t>(quarter * 32) << 16), v);
-        // (a cluster's CTA keeps it in its own shared memory, where the ring was: its only chain
-        // is over, so every load and product of the ring is)
-        float* p = (plan.cluster ? reinterpret_cast<float*>(smem) : part) +
-                   (static_cast<int64_t>(c / 32) * 4 + quarter) * 1024 + lane * 4;
+        if (cluster) {
+          // a cluster's CTA keeps it in its own shared memory, where the ring was (its only
+          // chain is over, so every load and product of the ring is), row by row, pieces of 4
+          // columns swizzled
+          float4* t = reinterpret_cast<float4*>(smem) + (quarter * 32 + lane) * 32;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            t[(c / 4 + j) ^ lane] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          continue;
+        }
+        float* p = part + (static_cast<int64_t>(c / 32) * 4 + quarter) * 1024 + lane * 4;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (chunk == 0)
@@ -325,22 +337,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
-  if (plan.cluster) {
+  if (cluster) {
     // gW (+)= the cluster's partial tiles, in order, each CTA a share of the tile
     cluster_sync();
-    constexpr int kQuads = 128 * MT * NT / 4;
+    // (a warp 128 columns of a row: whole lines of gW)
+    constexpr int kQuads = 128 * 128 / 4;
     const int splits = kb_total > 0 ? sh.splits : 0;
     for (int x = split * kThreads + static_cast<int>(threadIdx.x); x < kQuads; x += plan.splits * kThreads) {
+      const int row = x / 32, k = x % 32;
+      const uint8_t* at = smem + (row * 32 + (k ^ (row & 31))) * 16;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       float4 v[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < splits) v[r] = ld_cluster4(cluster_addr(smem + x * 16, static_cast<uint32_t>(r)));
+        if (r < splits) v[r] = ld_cluster4(cluster_addr(at, static_cast<uint32_t>(r)));
       }
 #pragma unroll
       for (int r = 0; r < 8; ++r) s.x += v[r].x, s.y += v[r].y, s.z += v[r].z, s.w += v[r].w;
-      add_quad(a, plan, tile, x * 4, s);
+      add_quad(a, m0 + row, n0 + k * 4, s);
     }
     cluster_sync();  // the others may still read this CTA's tile
   }
@@ -667,7 +682,11 @@ __global__ void __launch_bounds__(256) ckpt8_dw_sum_kernel(Ckpt8DwArgs a, DwPlan
     s.z += v.z;
     s.w += v.w;
   }
-  add_quad(a, plan, tile, at, s);
+  // at = ((c / 32) * 4 + quarter) * 1024 + j * 128 + lane * 4, c the column over the accumulators
+  const int lane = (at / 4) % 32, j = (at / 128) % 8, quarter = (at / 1024) % 4;
+  const int c = (at / 4096) * 32 + j * 4;
+  add_quad(a, (tile / plan.n_tiles) * 128 * plan.mt + (c / plan.nt) * 128 + quarter * 32 + lane,
+           (tile % plan.n_tiles) * plan.nt + c % plan.nt, s);
 }
 
 // Tile and shares for M x N over cap rows on num_sms SMs.  The large tile (256 x 256) reads
