@@ -76,14 +76,6 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // TMA store of one [box rows][64 cols] bf16 panel from 128B-swizzled shared memory.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem_src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -196,7 +188,8 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
 // tensor memory that has been read (tcgen05.wait::ld and the fence before it) or shared
 // memory written through fence.proxy.async, so the default scope is enough on both sides;
 // with .release.cluster here and .acquire.cluster on the wait, every hand-over also waited
-// for the warp's global stores (measured: the weight gradient 286 us instead of PAIR_US).
+// for the warp's global stores (linear 139058 x 512 x 256 with GELU and 8-bit z: 57.9 us
+// instead of 51.9).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -241,28 +234,6 @@ inline CUtensorMap tensor_map_bf16(const void* ptr, int64_t rows, int64_t cols, 
 inline CUtensorMap tensor_map_u8(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows,
                                  CUtensorMapSwizzle swizzle) {
   return tensor_map_2d(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ptr, rows, cols, ld, box_cols, box_rows, swizzle);
-}
-
-// The same matrix as [cols / box_cols][rows][box_cols], 128B swizzle: one load brings
-// box_blocks column blocks, each in the layout of a 2D box.  cols is a multiple of
-// box_cols (a block past it would read past the row).
-inline CUtensorMap tensor_map_blocks(CUtensorMapDataType type, int esize, const void* ptr, int64_t rows, int64_t cols,
-                                     int64_t ld, int box_cols, int box_rows, int box_blocks) {
-  if ((reinterpret_cast<uintptr_t>(ptr) & 15u) != 0) throw std::invalid_argument("TMA operand not 16-byte aligned");
-  if ((ld * esize) % 16 != 0) throw std::invalid_argument("TMA operand row stride must be a multiple of 16 bytes");
-  if (cols % box_cols != 0) throw std::invalid_argument("column blocks need whole blocks");
-  CUtensorMap m;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(box_cols), static_cast<cuuint64_t>(rows > 0 ? rows : 1),
-                        static_cast<cuuint64_t>(cols / box_cols)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * esize), static_cast<cuuint64_t>(box_cols) * esize};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows),
-                       static_cast<cuuint32_t>(box_blocks)};
-  cuuint32_t estr[3] = {1u, 1u, 1u};
-  CUresult r = tensor_map_encoder()(&m, type, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string(static_cast<int>(r)));
-  return m;
 }
 
 // opt the kernel into `bytes` of dynamic shared memory on the current device (once per

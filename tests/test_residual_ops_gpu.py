@@ -305,7 +305,9 @@ def test_rmsnorm_zero_rows_and_huge_rows():
 # ------------------------------------------------------------------ linear
 LINEAR = [(1, 1, 8, 1), (3, 5, 16, 8), (31, 40, 24, 47), (127, 130, 64, 64), (129, 129, 100, 65), (200, 256, 208, 256),
           (1000, 3000, 512, 256), (1000, 20000, 72, 200), (20000, 20000, 40, 300), (257, 300, 1032, 129), (0, 10, 16, 16),
-          (19000, 19000, 136, 136), (2000, 2001, 256, 1000)]
+          (19000, 19000, 136, 136), (2000, 2001, 256, 1000),
+          # enough products for the 256-column tiles of CTA pairs
+          (75001, 75100, 200, 136), (8000, 8100, 1032, 520), (300, 20000, 1024, 256), (4097, 4200, 2056, 300)]
 
 
 @pytest.mark.parametrize("n,cap,k,m", LINEAR)
@@ -466,7 +468,10 @@ def test_linear_act_bwd_draws_the_forward_mask():
                                        (2048, 2048, 1000, 300),
                                        # enough rows for the 256 x 256 tiles of CTA pairs
                                        (40003, 40100, 300, 300), (152064, 152064, 512, 256), (160001, 170000, 136, 200),
-                                       (40960, 41000, 520, 264)])
+                                       (40960, 41000, 520, 264),
+                                       # few live rows of many in a cluster; several chains a share
+                                       (100, 2048, 512, 256), (1999, 2000, 300, 65), (90000, 90010, 520, 100),
+                                       (200001, 200064, 1000, 64)])
 @pytest.mark.parametrize("wide", [0, 64])
 def test_ckpt8_dw(n, cap, k, m, wide):
     g = gen_for("dw", n, k, m)
