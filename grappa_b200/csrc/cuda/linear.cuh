@@ -39,10 +39,15 @@ namespace {
 constexpr int BM = 128;
 constexpr int BK = 64;
 
-// A warp of the epilogue owns 32 rows x 64 columns of the tile: one panel of output /
+// A warp of the epilogue owns 32 rows x 64 columns of the tile, in two half panels of output /
 // residual.  The 256-wide tile takes a whole SM (16 epilogue warps);
-// narrower tiles share it (2 and 3 CTAs), so that as many warps work on epilogues.
-template <int BN, int CG>
+// narrower tiles share it (2 and 3 CTAs), so that as many warps work on epilogues.  What the
+// epilogue needs no room for (RES: residuals, Q8: codes) goes to the ring: a load takes some
+// 2000 cycles under load, a stage's products 640 (131072 x 1024 x 1024: 263 / 224 / 215 us
+// with 3 / 4 / 5 stages).  With codes, though, a second half panel is worth more than a fifth
+// stage unless the products are long (139058 x 208 x 256 with GELU 39.4 / 41.5 us, 65536 x
+// 1024 x 512 74 / 71).
+template <int BN, int CG, bool RES, bool Q8>
 struct LSmem {
   static constexpr int kEpi = BN / 16;                       // epilogue warps
   static constexpr int kCtas = BN == 256 ? 1 : (BN == 128 ? 2 : 3);
@@ -51,11 +56,13 @@ struct LSmem {
   static constexpr int kBRows = BN / CG;                     // a pair of CTAs shares W's tile
   static constexpr int kBBytes = kBRows * BK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kOutBytes = kEpi * 4096;              // a 32 x 64 bf16 panel a warp
-  static constexpr bool kCodePanel = CG == 2;                // and a 32 x 64 panel of codes
+  static constexpr int kPanels = CG == 2 && !RES && !Q8 ? 1 : 2;  // of 32 x 32 bf16 a warp
+  static constexpr int kOutBytes = kEpi * kPanels * 2048;
+  static constexpr bool kCodePanel = CG == 2 && Q8;          // and a 32 x 64 panel of codes
   static constexpr int kCodeBytes = kCodePanel ? kEpi * 2048 : 0;
   static constexpr int kBudget = 226 * 1024 / kCtas - 2048 - kOutBytes - kCodeBytes;
-  static constexpr int kStages = kBudget / kStageBytes > 4 ? 4 : kBudget / kStageBytes;
+  static constexpr int kMost = CG == 2 ? 6 : 4;
+  static constexpr int kStages = kBudget / kStageBytes > kMost ? kMost : kBudget / kStageBytes;
   static constexpr int kTmemCols = 2 * BN;
   static constexpr int kBytes = kStages * kStageBytes + kOutBytes + kCodeBytes + 1024 /*align*/;
   static_assert(kStages >= 2 && kCtas * (kBytes + 512) <= 227 * 1024 && kCtas * kTmemCols <= 512, "linear: resources");
@@ -74,11 +81,11 @@ __device__ __forceinline__ uint2 codes8_relu(const float* v, float inv) {
 }
 
 template <int BN, int CG, int ACT, bool RES, bool Q8, bool ANY>
-__global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
+__global__ void __launch_bounds__(LSmem<BN, CG, true, true>::kThreads, LSmem<BN, CG, true, true>::kCtas)
     linear_fwd_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                       const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmO,
                       const __grid_constant__ CUtensorMap tmQ, LinearArgs a) {
-  using S = LSmem<BN, CG>;
+  using S = LSmem<BN, CG, RES || ANY, Q8 || ANY>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2], res_full[S::kEpi][2];
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
     const int w = warp - 2;
     const int quarter = warp & 3;  // TMEM lanes that this warp may read
     const int col0 = (w / 4) * 64;
-    uint8_t* panels = out_area + w * 4096;  // two of 32 rows x 32 columns
+    uint8_t* panels = out_area + w * (S::kPanels * 2048);  // of 32 rows x 32 columns
     uint8_t* codes = code_area + w * 2048;
     const uint64_t key = ANY && a.dropout_p > 0.f ? hop_key(static_cast<uint64_t>(a.counters[0]) ^ 0xD80Full,
                                                             static_cast<uint64_t>(a.counters[1]),
@@ -262,14 +269,14 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
         const int nc = nc0 + h * 32;
         const bool whole = nc + 32 <= a.N;
         const bool code_cols = nc < n_code;
-        uint8_t* panel = panels + h * 2048;
+        uint8_t* panel = panels + (S::kPanels == 2 ? h * 2048 : 0);
         float v[32];
         tmem_ld32(trow + h * 32, v);
         if (lane == 0) {
-          // what is written below has left: this half's panel, two stores ago; with a residual
-          // the other half's panel too, into which the next residual comes while this one is
-          // used; the code panel, a store ago
-          if (has_res || (S::kCodePanel && has_q8 && h == 0)) {
+          // what is written below has left: this half's panel, two stores ago (a store ago, where
+          // there is one panel); with a residual the other half's panel too, into which the next
+          // residual comes while this one is used; the code panel, a store ago
+          if (has_res || S::kPanels == 1 || (S::kCodePanel && has_q8 && h == 0)) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             if (has_res && h == 0) ask(t, 1);
             if (has_res && h == 1 && t + step < tiles) ask(t + step, 0);
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(LSmem<BN, CG>::kThreads, LSmem<BN, CG>::kCtas)
 
 template <int BN, int CG, int ACT, bool RES, bool Q8, bool ANY>
 void linear_kernel(const LinearArgs& a, cudaStream_t stream) {
-  using S = LSmem<BN, CG>;
+  using S = LSmem<BN, CG, RES || ANY, Q8 || ANY>;
   const int64_t n_pad = ceil_div(a.N, 8) * 8;
   const CUtensorMap ma = tensor_map_bf16(a.A, a.a_rows, a.K, a.lda, BM);
   const CUtensorMap mw = tensor_map_bf16(a.W, a.N, a.K, a.ldw, S::kBRows);
