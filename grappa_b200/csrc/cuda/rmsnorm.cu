@@ -8,10 +8,12 @@
 //
 // Each row is read once and each output written once; a dozen operations an element, so
 // HBM bounds both.  A team of lanes holds a row in registers, eight columns (one or two
-// 16-byte loads) a lane, two rows at a time: 4 to 32 lanes for rows of up to 256 columns, two
-// to eight warps up to 2048, a whole CTA with two or four steps above.  The row sums are
-// shuffles, and one shared-memory exchange for teams of several warps.  All sums and
-// statistics are fp32.
+// 16-byte loads) a lane: 4 to 32 lanes for rows of up to 256 columns, two to eight warps up to
+// 2048, a whole CTA with two or four steps above.  Loads are kept in flight by two rows at a
+// time (forward) or by asking for the next row early (backward).  The row sums are shuffles,
+// and one shared-memory exchange for teams of several warps.  All sums and statistics are fp32.
+// Measured: forward 139058 x 256 bf16 with residual and 8-bit rows 52.7 us, 94 % of the copy's
+// rate; backward 1000003 x 128 from 8-bit rows 155 us, 90 %; 139058 x 256 bf16 49 us, 90 %.
 //
 // dgamma: a lane sums its columns over the rows of its team, the CTA joins its teams in
 // shared memory in a fixed order and writes one part, and a second kernel sums the parts
@@ -191,8 +193,13 @@ __global__ void __launch_bounds__(kThreads, NV * R <= 2 ? 4 : 2) rmsnorm_fwd_ker
   }
 }
 
+// CTAs of the backward kernel that an SM holds
+constexpr int bwd_ctas(int ky, int kx, int kd, int nv) {
+  return nv > 1 ? 1 : (ky == kF32 || kx == kF32 || kd == kF32 ? 3 : 4);
+}
+
 template <int KY, int KX, int KD, int TEAM, int NV, int R>
-__global__ void __launch_bounds__(kThreads, NV > 1 ? 1 : (KY == kF32 || KX == kF32 || KD == kF32 ? 2 : 3))
+__global__ void __launch_bounds__(kThreads, bwd_ctas(KY, KX, KD, NV))
     rmsnorm_bwd_kernel(RmsNormBwdArgs a) {
   GB_PDL_ENTRY();
   __shared__ float sh[R][8];
@@ -214,17 +221,17 @@ __global__ void __launch_bounds__(kThreads, NV > 1 ? 1 : (KY == kF32 || KX == kF
       gam[i][j] = col < a.dim ? a.gamma[col] : 0.f;
     }
   }
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * R; base < n;
-       base += static_cast<int64_t>(gridDim.x) * kTeams * R) {
-    Raw8<KY> yr[R][NV];
-    Raw8<KX> xr[R][NV];
-    Raw8<KD> rr[R][NV];
-    uint32_t eb[R][NV];
-    float rs[R];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTeams * R;
+  Raw8<KY> yr[R][NV];
+  Raw8<KX> xr[R][NV];
+  Raw8<KD> rr[R][NV];
+  uint32_t eb[R][NV];
+  float rs_next[R];
+  auto fetch = [&](int64_t base) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = base + r * kTeams + team;
-      rs[r] = row < n ? a.rstd[row] : 0.f;
+      rs_next[r] = row < n ? a.rstd[row] : 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = i * TEAM + t;
@@ -240,15 +247,27 @@ __global__ void __launch_bounds__(kThreads, NV > 1 ? 1 : (KY == kF32 || KX == kF
         rr[r][i] = on && row < n_res ? raw_load<KD>(a.dres, row * a.lddr + c * 8) : raw_zero<KD>();
       }
     }
-    float dy[R][NV][8], xh[R][NV][8], dot[R];
+  };
+  // The next rows are asked for as soon as these are in fp32 (wider rows have no registers
+  // left for that): 1000003 x 128 from 8-bit rows with a residual, two rows at a time and three
+  // CTAs an SM 171 us, so with one row and four CTAs 155
+  constexpr bool kFetchAhead = NV == 1;
+  const int64_t base0 = static_cast<int64_t>(blockIdx.x) * kTeams * R;
+  if (kFetchAhead) fetch(base0);
+  for (int64_t base = base0; base < n; base += step) {
+    if (!kFetchAhead) fetch(base);
+    float dy[R][NV][8], xh[R][NV][8], dot[R], rs[R];
+    Raw8<KD> dr_raw[R][NV];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       dot[r] = 0.f;
+      rs[r] = rs_next[r];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = i * TEAM + t;
         raw_values<KY>(yr[r][i], 0.f, dy[r][i]);
         raw_values<KX>(xr[r][i], group8_scale(eb[r][i]), xh[r][i]);
+        dr_raw[r][i] = rr[r][i];
         mask8(dy[r][i], c, a.dim);
         mask8(xh[r][i], c, a.dim);
 #pragma unroll
@@ -260,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, NV > 1 ? 1 : (KY == kF32 || KX == kF
         }
       }
     }
+    if (kFetchAhead && base + step < n) fetch(base + step);
     team_sum<TEAM, R>(dot, sh);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -270,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, NV > 1 ? 1 : (KY == kF32 || KX == kF
         const int c = i * TEAM + t;
         if (row < n && c < chunks) {
           float dr[8], o[8];
-          raw_values<KD>(rr[r][i], 0.f, dr);
+          raw_values<KD>(dr_raw[r][i], 0.f, dr);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             o[j] = fmaf(rs[r], fmaf(-xh[r][i][j], mean, gam[i][j] * dy[r][i][j]), dr[j]);
@@ -335,7 +355,7 @@ __global__ void __launch_bounds__(1024)
 // CTAs for cap rows: one pass of rows each, up to as many as the SMs hold at once.  Few rows
 // are left to one cluster of up to eight CTAs, which joins its column sums over distributed
 // shared memory: no second kernel, no work area (4.8 against 8.1 us a call for 64 x 64 rows).
-constexpr int kBwdCtasPerSm = 3;
+constexpr int kBwdPasses = 2 * kClusterPasses;
 template <int TEAM, int R>
 int64_t passes(int cap) { return std::max<int64_t>(1, ceil_div(cap, kThreads / TEAM * R)); }
 
@@ -365,14 +385,14 @@ void bwd_t(RmsNormBwdArgs a, int num_sms, cudaStream_t stream) {
   const int64_t want = passes<TEAM, R>(a.cap);
   const size_t smem = sizeof(float) * ((TEAM < kThreads ? kThreads * NV * 8 : 0) + TEAM * NV * 8);
   auto kern = rmsnorm_bwd_kernel<KY, KX, KD, TEAM, NV, R>;
-  if (want <= kClusterPasses) {
+  if (want <= kBwdPasses) {
     a.cluster = true;
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(want, 8));
     launch_cluster_k(kern, dim3(grid), dim3(kThreads), grid, smem, stream, a);
     GB_LAUNCH_CHECK();
     return;
   }
-  const int grid = static_cast<int>(std::min<int64_t>(want, static_cast<int64_t>(num_sms) * kBwdCtasPerSm));
+  const int grid = static_cast<int>(std::min<int64_t>(want, static_cast<int64_t>(num_sms) * bwd_ctas(KY, KX, KD, NV)));
   launch_k(kern, dim3(grid), dim3(kThreads), smem, stream, a);
   GB_LAUNCH_CHECK();
   launch_sum_parts(a.work, grid, a.dim, a.dim, a.dgamma, a.accumulate, stream);
@@ -381,12 +401,12 @@ void bwd_t(RmsNormBwdArgs a, int num_sms, cudaStream_t stream) {
 template <int KY, int KX, int KD>
 void bwd_k(const RmsNormBwdArgs& a, int num_sms, cudaStream_t stream) {
   const int d = a.dim;
-  if (d <= 64) return bwd_t<KY, KX, KD, 8, 1, 2>(a, num_sms, stream);
-  if (d <= 128) return bwd_t<KY, KX, KD, 16, 1, 2>(a, num_sms, stream);
-  if (d <= 256) return bwd_t<KY, KX, KD, 32, 1, 2>(a, num_sms, stream);
-  if (d <= 512) return bwd_t<KY, KX, KD, 64, 1, 2>(a, num_sms, stream);
-  if (d <= 1024) return bwd_t<KY, KX, KD, 128, 1, 2>(a, num_sms, stream);
-  if (d <= 2048) return bwd_t<KY, KX, KD, 256, 1, 2>(a, num_sms, stream);
+  if (d <= 64) return bwd_t<KY, KX, KD, 8, 1, 1>(a, num_sms, stream);
+  if (d <= 128) return bwd_t<KY, KX, KD, 16, 1, 1>(a, num_sms, stream);
+  if (d <= 256) return bwd_t<KY, KX, KD, 32, 1, 1>(a, num_sms, stream);
+  if (d <= 512) return bwd_t<KY, KX, KD, 64, 1, 1>(a, num_sms, stream);
+  if (d <= 1024) return bwd_t<KY, KX, KD, 128, 1, 1>(a, num_sms, stream);
+  if (d <= 2048) return bwd_t<KY, KX, KD, 256, 1, 1>(a, num_sms, stream);
   if (d <= 4096) return bwd_t<KY, KX, KD, 256, 2, 1>(a, num_sms, stream);
   return bwd_t<KY, KX, KD, 256, 4, 1>(a, num_sms, stream);
 }
@@ -412,9 +432,9 @@ void launch_sum_parts(const float* part, int parts, int64_t ld, int cols, float*
 
 int64_t rmsnorm_bwd_work_floats(int dim, int cap, int num_sms) {
   // rows of a CTA's pass, as bwd_k takes them
-  const int rows = dim <= 64 ? 64 : dim <= 128 ? 32 : dim <= 256 ? 16 : dim <= 512 ? 8 : dim <= 1024 ? 4 : dim <= 2048 ? 2 : 1;
+  const int rows = dim <= 64 ? 32 : dim <= 128 ? 16 : dim <= 256 ? 8 : dim <= 512 ? 4 : dim <= 1024 ? 2 : 1;
   const int64_t want = ceil_div(std::max(cap, 1), rows);
-  return want <= kClusterPasses ? 0 : dim * std::min<int64_t>(want, static_cast<int64_t>(num_sms) * kBwdCtasPerSm);
+  return want <= kBwdPasses ? 0 : dim * std::min<int64_t>(want, static_cast<int64_t>(num_sms) * bwd_ctas(kBf, kBf, kBf, 1));
 }
 
 void launch_rmsnorm_fwd(const RmsNormArgs& a, int num_sms, cudaStream_t stream) {
