@@ -60,47 +60,58 @@ __global__ void __launch_bounds__(kThreads, 4) ckpt8_store_kernel(Ckpt8Args a) {
   }
 }
 
+// LPR lanes x 16 columns cover a row; a lane's 16 columns are pieces of 16 output bytes LPR
+// pieces apart, so that a store writes whole lines (sixteen neighbouring columns a lane, in
+// half and quarter sectors: 65537 x 992 to fp32 LOAD_OLD us instead of LOAD_NEW)
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads, 4) ckpt8_load_kernel(Ckpt8Args a) {
   GB_PDL_ENTRY();
   constexpr int kTeams = kThreads / LPR;
+  constexpr int kCols = 16 / sizeof(T), kPieces = 16 / kCols;
   const int n = live_rows(a.n_ptr, a.cap);
   const int t = threadIdx.x % LPR, team = threadIdx.x / LPR;
-  const int c = (blockIdx.y * LPR + t) * 16;
-  if (c >= a.dim) return;
+  const int c0 = blockIdx.y * LPR * 16 + t * kCols;
+  const int cols = (a.dim + 7) / 8 * 8;  // zeros from dim on
+  using Codes = std::conditional_t<kCols == 8, uint2, uint32_t>;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * kRowsC; base < n;
        base += static_cast<int64_t>(gridDim.x) * kTeams * kRowsC) {
-    uint4 q[kRowsC];
-    uint32_t e[kRowsC];
+    Codes q[kRowsC][kPieces];
+    uint32_t e[kRowsC][kPieces];
 #pragma unroll
     for (int r = 0; r < kRowsC; ++r) {
       const int64_t row = base + r * kTeams + team;
-      q[r] = make_uint4(0u, 0u, 0u, 0u);
-      e[r] = 0u;
-      if (row < n) {
-        q[r] = *reinterpret_cast<const uint4*>(a.q8.q + row * a.q8.ldq + c);
-        e[r] = a.q8.e[row * a.q8.lde + (c >> 5)];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int c = c0 + i * LPR * kCols;
+        q[r][i] = Codes();
+        e[r][i] = 0u;
+        if (row < n && c < cols) {
+          q[r][i] = *reinterpret_cast<const Codes*>(a.q8.q + row * a.q8.ldq + c);
+          e[r][i] = a.q8.e[row * a.q8.lde + (c >> 5)];
+        }
       }
     }
 #pragma unroll
     for (int r = 0; r < kRowsC; ++r) {
       const int64_t row = base + r * kTeams + team;
-      if (row >= n) continue;
-      T* p = static_cast<T*>(a.out) + row * a.ld + c;
-      if (sizeof(T) == 2 && c + 16 <= a.dim) {
-        const __nv_bfloat162 scale = group8_scale_bf16(e[r]);
-        *reinterpret_cast<uint4*>(p) = values8_bf16(q[r].x, q[r].y, scale);
-        *reinterpret_cast<uint4*>(p + 8) = values8_bf16(q[r].z, q[r].w, scale);
-      } else {
-        float v[8];
-        values8(make_uint2(q[r].x, q[r].y), group8_scale(e[r]), v);
-        mask8(v, c >> 3, a.dim);
-        store8(p, v);
-        if (c + 8 < a.dim) {
-          values8(make_uint2(q[r].z, q[r].w), group8_scale(e[r]), v);
-          mask8(v, (c >> 3) + 1, a.dim);
-          store8(p + 8, v);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int c = c0 + i * LPR * kCols;
+        if (row >= n || c >= cols) continue;
+        uint4 o;
+        if constexpr (kCols == 8) {
+          o = values8_bf16(q[r][i].x, q[r][i].y, group8_scale_bf16(e[r][i]));
+        } else {
+          float v[4];
+          values4(q[r][i], group8_scale(e[r][i]), v);
+          o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
         }
+        if (c + kCols > a.dim) {
+          const int k = a.dim - c;
+          o = kCols == 8 ? first_columns(o, k)
+                         : make_uint4(k > 0 ? o.x : 0u, k > 1 ? o.y : 0u, k > 2 ? o.z : 0u, 0u);
+        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ld + c) = o;
       }
     }
   }

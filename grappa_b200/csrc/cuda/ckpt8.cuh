@@ -66,18 +66,21 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ float abs_max8(const float* v) {
   return max_nan(abs_max3(abs_max3(v[0], v[1], v[2]), v[3], v[4]), abs_max3(v[5], v[6], v[7]));
 }
-// the eight values of a chunk's codes: a code c + 128 in the low byte of 2^23 is the float
+// the four values of a word's codes: a code c + 128 in the low byte of 2^23 is the float
 // 8388736 + c (a byte permutation instead of the quarter-rate integer conversion)
-__device__ __forceinline__ void values8(uint2 q, float scale, float* v) {
-  q.x ^= 0x80808080u;
-  q.y ^= 0x80808080u;
+__device__ __forceinline__ void values4(uint32_t q, float scale, float* v) {
+  q ^= 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const uint32_t w = i < 4 ? q.x : q.y;
-    const F2 c = f2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + (i & 3))),
-                    __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7541 + (i & 3))));
+  for (int i = 0; i < 4; i += 2) {
+    const F2 c = f2(__uint_as_float(__byte_perm(q, 0x4B000000u, 0x7540 + i)),
+                    __uint_as_float(__byte_perm(q, 0x4B000000u, 0x7541 + i)));
     unpack(mul2(add2(c, both(-8388736.f)), both(scale)), v[i], v[i + 1]);
   }
+}
+// the eight values of a chunk's codes
+__device__ __forceinline__ void values8(uint2 q, float scale, float* v) {
+  values4(q.x, scale, v);
+  values4(q.y, scale, v + 4);
 }
 // The same as four bf16 pairs, without passing through fp32: with x = c + 128 = 128 h + m (m of
 // seven bits), c = (128 + m) - (256 - 128 h); both terms are bf16 patterns made by one logic
