@@ -2,7 +2,7 @@
 //
 // All three are one pass over their rows with a few operations an element (the
 // activation's slope: an exponential and a division), so HBM bounds them.  A lane takes
-// sixteen columns of a row (eight in the activation backward), and several rows in flight.
+// eight or sixteen columns of a row, several loads in flight.
 #include <algorithm>
 #include <type_traits>
 
@@ -18,43 +18,71 @@ namespace dev {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowsC = 2;  // rows a thread has in flight
+constexpr int kRowsC = 2;  // rows a thread of the load kernel has in flight
+// pieces of 16 bytes that a thread of the store kernel has in flight, and its CTAs an SM:
+// 139058 x 512 bf16 with 2 pieces and 4 / 6 CTAs 40.3 / 35.4 us (94 % of the copy's rate), with 4
+// pieces 40.7 (sixteen neighbouring columns a lane took 41)
+template <typename T>
+constexpr int kInFlight = sizeof(T) == 2 ? 2 : 4;
+constexpr int kStoreCtas = 6;
 
-// LPR lanes x 16 columns cover a row (blockIdx.y the next LPR * 16 columns of wide rows);
-// lanes 2i and 2i + 1 hold a group.
-template <typename T, int LPR>
-__global__ void __launch_bounds__(kThreads, 4) ckpt8_store_kernel(Ckpt8Args a) {
+// LPR lanes x P pieces of 16 bytes cover a row (blockIdx.y the next of wide rows); pieces of a
+// lane lie LPR apart, so that loads and code stores are whole lines, and a group's pieces in
+// neighbouring lanes.
+template <typename T>
+constexpr int kPieceCols = 16 / sizeof(T);
+template <typename T, int LPR, int P>
+__global__ void __launch_bounds__(kThreads, kStoreCtas) ckpt8_store_kernel(Ckpt8Args a) {
   GB_PDL_ENTRY();
-  constexpr int kTeams = kThreads / LPR;
+  constexpr int kTeams = kThreads / LPR, kCols = kPieceCols<T>, kGroup = 32 / kCols, R = kInFlight<T> / P;
+  static_assert(LPR % kGroup == 0, "groups in neighbouring lanes");
   const int n = live_rows(a.n_ptr, a.cap);
   const int t = threadIdx.x % LPR, team = threadIdx.x / LPR;
-  const int c = (blockIdx.y * LPR + t) * 16;  // first column
-  const bool in = c < (a.dim + 31) / 32 * 32;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * kRowsC; base < n;
-       base += static_cast<int64_t>(gridDim.x) * kTeams * kRowsC) {
-    float v[kRowsC][16];
+  const int c0 = (blockIdx.y * P * LPR + t) * kCols;
+  const int q_cols = (a.dim + 31) / 32 * 32;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTeams * R; base < n;
+       base += static_cast<int64_t>(gridDim.x) * kTeams * R) {
+    uint4 raw[R][P];
 #pragma unroll
-    for (int r = 0; r < kRowsC; ++r) {
+    for (int r = 0; r < R; ++r) {
       const int64_t row = base + r * kTeams + team;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[r][j] = 0.f;
-      const T* p = static_cast<const T*>(a.x) + row * a.ld + c;
-      if (row < n && c < a.dim) load8(p, v[r]);
-      if (row < n && c + 8 < a.dim) load8(p + 8, v[r] + 8);
+      for (int i = 0; i < P; ++i) {
+        const int c = c0 + i * LPR * kCols;
+        raw[r][i] = row < n && c < a.dim
+                        ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ld + c)
+                        : make_uint4(0u, 0u, 0u, 0u);
+      }
     }
 #pragma unroll
-    for (int r = 0; r < kRowsC; ++r) {
+    for (int r = 0; r < R; ++r) {
       const int64_t row = base + r * kTeams + team;
-      mask8(v[r], c >> 3, a.dim);
-      mask8(v[r] + 8, (c >> 3) + 1, a.dim);
-      float m = max_nan(abs_max8(v[r]), abs_max8(v[r] + 8));
-      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      const uint32_t byte = group8_byte(m);
-      const float inv = group8_inv(byte);
-      if (row < n && in) {
-        const uint2 q0 = codes8(v[r], inv), q1 = codes8(v[r] + 8, inv);
-        *reinterpret_cast<uint4*>(a.q8.q + row * a.q8.ldq + c) = make_uint4(q0.x, q0.y, q1.x, q1.y);
-        if ((t & 1) == 0) a.q8.e[row * a.q8.lde + (c >> 5)] = static_cast<uint8_t>(byte);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int c = c0 + i * LPR * kCols;
+        if (c + kCols > a.dim) raw[r][i] = first_columns<T>(raw[r][i], a.dim - c);
+        float v[8];
+        float m;
+        if constexpr (kCols == 8) {
+          bf16x8_to_f32(raw[r][i], v);
+          m = abs_max8(v);
+        } else {
+          v[0] = __uint_as_float(raw[r][i].x), v[1] = __uint_as_float(raw[r][i].y);
+          v[2] = __uint_as_float(raw[r][i].z), v[3] = __uint_as_float(raw[r][i].w);
+          m = max_nan(abs_max3(fabsf(v[0]), v[1], v[2]), fabsf(v[3]));
+        }
+#pragma unroll
+        for (int o = 1; o < kGroup; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const uint32_t byte = group8_byte(m);
+        const float inv = group8_inv(byte);
+        if (row < n && c < q_cols) {
+          int8_t* q = a.q8.q + row * a.q8.ldq + c;
+          if constexpr (kCols == 8)
+            *reinterpret_cast<uint2*>(q) = codes8(v, inv);
+          else
+            *reinterpret_cast<uint32_t*>(q) = codes4(v, inv);
+          if (t % kGroup == 0) a.q8.e[row * a.q8.lde + (c >> 5)] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
@@ -62,7 +90,8 @@ __global__ void __launch_bounds__(kThreads, 4) ckpt8_store_kernel(Ckpt8Args a) {
 
 // LPR lanes x 16 columns cover a row; a lane's 16 columns are pieces of 16 output bytes LPR
 // pieces apart, so that a store writes whole lines (sixteen neighbouring columns a lane, in
-// half and quarter sectors: 65537 x 992 to fp32 LOAD_OLD us instead of LOAD_NEW)
+// half and quarter sectors: 65537 x 992 to fp32 80 us instead of 58, 139058 x 512 to bf16 38
+// instead of 35: 94 % of the copy's rate)
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads, 4) ckpt8_load_kernel(Ckpt8Args a) {
   GB_PDL_ENTRY();
@@ -106,15 +135,30 @@ __global__ void __launch_bounds__(kThreads, 4) ckpt8_load_kernel(Ckpt8Args a) {
           values4(q[r][i], group8_scale(e[r][i]), v);
           o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
         }
-        if (c + kCols > a.dim) {
-          const int k = a.dim - c;
-          o = kCols == 8 ? first_columns(o, k)
-                         : make_uint4(k > 0 ? o.x : 0u, k > 1 ? o.y : 0u, k > 2 ? o.z : 0u, 0u);
-        }
+        if (c + kCols > a.dim) o = first_columns<T>(o, a.dim - c);
         *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ld + c) = o;
       }
     }
   }
+}
+
+template <typename T, int LPR, int P>
+void store_t(const Ckpt8Args& a, cudaStream_t stream) {
+  const int64_t passes = ceil_div(a.cap, kThreads / LPR * (kInFlight<T> / P));
+  const int64_t slices = ceil_div(ceil_div(a.dim, 32) * 32, LPR * P * kPieceCols<T>);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(passes, ceil_div(sm_count() * kStoreCtas, slices))),
+                  static_cast<unsigned>(slices));
+  launch_k(ckpt8_store_kernel<T, LPR, P>, grid, dim3(kThreads), 0, stream, a);
+  GB_LAUNCH_CHECK();
+}
+template <typename T>
+void store_rows(const Ckpt8Args& a, cudaStream_t stream) {
+  constexpr int kCols = kPieceCols<T>;
+  if (a.dim <= 32) return store_t<T, 32 / kCols, 1>(a, stream);
+  if (a.dim <= 64) return store_t<T, 64 / kCols, 1>(a, stream);
+  if (a.dim <= 128) return store_t<T, 128 / kCols, 1>(a, stream);
+  if (a.dim <= 256) return store_t<T, 32, 8 / kCols>(a, stream);
+  return store_t<T, 32, 16 / kCols>(a, stream);
 }
 
 // calls f with the lanes per row (a compile-time constant) for rows of `dim` columns
@@ -297,12 +341,7 @@ void launch_linear_act_bwd(LinearActBwdArgs a, int num_sms, cudaStream_t stream)
 
 void launch_ckpt8_store(const Ckpt8Args& a, cudaStream_t stream) {
   if (a.cap <= 0) return;
-  with_lpr(a.dim, [&](auto lpr) {
-    constexpr int L = decltype(lpr)::value;
-    launch_k(a.f32 ? ckpt8_store_kernel<float, L> : ckpt8_store_kernel<__nv_bfloat16, L>, ckpt_grid<L>(a.dim, a.cap),
-             dim3(kThreads), 0, stream, a);
-  });
-  GB_LAUNCH_CHECK();
+  a.f32 ? store_rows<float>(a, stream) : store_rows<__nv_bfloat16>(a, stream);
 }
 
 void launch_ckpt8_load(const Ckpt8Args& a, cudaStream_t stream) {

@@ -41,16 +41,18 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 }
 // eight codes of one chunk (a group's columns are four consecutive chunks); inv = 0, of a
 // group that is not finite, makes codes 0 of its finite values, and the others are masked
-__device__ __forceinline__ uint2 codes8(const float* v, float inv) {
-  uint32_t c[8];
+__device__ __forceinline__ uint32_t codes4(const float* v, float inv) {
+  uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
+  for (int i = 0; i < 4; i += 2) {
     float a, b;
     unpack(fma2(f2(v[i], v[i + 1]), both(inv), both(12582912.f)), a, b);
     c[i] = __float_as_uint(a), c[i + 1] = __float_as_uint(b);
   }
-  const uint32_t on = inv == 0.f ? 0u : 0xFFFFFFFFu;
-  return make_uint2(pack4(c[0], c[1], c[2], c[3]) & on, pack4(c[4], c[5], c[6], c[7]) & on);
+  return inv == 0.f ? 0u : pack4(c[0], c[1], c[2], c[3]);
+}
+__device__ __forceinline__ uint2 codes8(const float* v, float inv) {
+  return make_uint2(codes4(v, inv), codes4(v + 4, inv));
 }
 // max(|a|, |b|, |c|), NaN if one of them is
 __device__ __forceinline__ float abs_max3(float a, float b, float c) {
@@ -133,8 +135,10 @@ __device__ __forceinline__ void mask8(float* v, int c, int dim) {
     if (c * 8 + i >= dim) v[i] = 0.f;
 }
 
-// the first n of eight bf16 columns, zeros after them
+// the first n columns of 16 bytes, zeros after them
+template <typename T = __nv_bfloat16>
 __device__ __forceinline__ uint4 first_columns(uint4 o, int n) {
+  if constexpr (sizeof(T) == 4) return make_uint4(n > 0 ? o.x : 0u, n > 1 ? o.y : 0u, n > 2 ? o.z : 0u, n > 3 ? o.w : 0u);
   auto keep = [](uint32_t w, int k) { return k >= 2 ? w : (k == 1 ? w & 0xFFFFu : 0u); };
   return make_uint4(keep(o.x, n), keep(o.y, n - 2), keep(o.z, n - 4), keep(o.w, n - 6));
 }
