@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(1024)
 // CTAs for cap rows: one pass of rows each, up to as many as the SMs hold at once.  Few rows
 // are left to one cluster of up to eight CTAs, which joins its column sums over distributed
 // shared memory: no second kernel, no work area (4.8 against 8.1 us a call for 64 x 64 rows).
-constexpr int kBwdPasses = 2 * kClusterPasses;
+constexpr int kBwdPasses = 2 * kClusterPasses;  // a pass is one row a team, half of what others take
 template <int TEAM, int R>
 int64_t passes(int cap) { return std::max<int64_t>(1, ceil_div(cap, kThreads / TEAM * R)); }
 

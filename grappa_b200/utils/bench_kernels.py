@@ -4,7 +4,7 @@ fused all-reduce + Adam kernel on one rank (its local HBM side).  CUDA-event dev
 times after warm-up, inputs sized as in a training step of the ogbn-products-shaped
 workload (``--scale`` multiplies the row counts).
 
-    python -m grappa_b200.utils.bench_kernels [--scale 1] [--part gemm,aggregate,ar]
+    python -m grappa_b200.utils.bench_kernels [--scale 1] [--part gemm,aggregate,residual,ar]
 Prints one JSON line per measurement.
 """
 import argparse
@@ -275,10 +275,81 @@ def repart_case(n_part=600_000, deg=50, n_global=2_449_029, halo=400_000, dim=10
     return res
 
 
+def residual_cases(s=1.0, iters=20):
+    """The residual layer's operators, two sets of buffers in turn (together larger than L2
+    but for the small ones): time, bytes that have to move and products.  iters=1 runs each
+    once, without warm-up (for a profiler)."""
+    cu = _native.cuda()
+    dev = torch.device("cuda", 0)
+    bf, f32 = torch.bfloat16, torch.float32
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def rows(n, d, t=bf):
+        return torch.randn(n, d, device=dev).to(t)
+
+    def coded(n, d):
+        q = torch.randint(-127, 128, (n, d), dtype=torch.int8, device=dev)
+        return q, torch.full((n, d // 32), 120, dtype=torch.uint8, device=dev)
+
+    def norm(n, d):
+        g, r = torch.ones(d, device=dev), torch.zeros(n, device=dev)
+        sets = [(rows(n, d), rows(n, d), rows(n, d), rows(n, d), *coded(n, d)) for _ in range(2)]
+        return lambda x, res, so, y, q, e: cu.rmsnorm_fwd(x, d, None, n, g, 1e-5, y, r, residual=res, s_out=so, q=q,
+                                                          q_exp=e), sets, n * d * (8 + 33 / 32), 0
+
+    def norm_bwd(n, d):
+        g, r, dg = torch.ones(d, device=dev), torch.ones(n, device=dev), torch.zeros(d, device=dev)
+        sets = [(rows(n, d), *coded(n, d), rows(n, d), rows(n, d)) for _ in range(2)]
+        return lambda dy, q, e, dr, dx: cu.rmsnorm_bwd(dy, None, r, g, d, None, n, dx, dg, dres=dr, q=q,
+                                                       q_exp=e), sets, n * d * (6 + 33 / 32), 0
+
+    def linear(n, k, m):
+        w, b = (rows(m, k, f32) / math.sqrt(k)).to(bf), torch.zeros(m, device=dev)
+        sets = [(rows(n, k), rows(n, m), rows(n, m), *coded(n, m)) for _ in range(2)]
+        return lambda x, res, out, q, e: cu.linear_fwd(x, w, None, n, out, err, bias=b, act=3, residual=res, q=q,
+                                                       q_exp=e), sets, n * (2 * k + 4 * m + m * 33 / 32), 2 * n * k * m
+
+    def act_bwd(n, d):
+        db = torch.zeros(d, device=dev)
+        sets = [(rows(n, d, f32), rows(n, d), *coded(n, d)) for _ in range(2)]
+        return lambda g, dz, q, e: cu.linear_act_bwd(g, d, None, n, 2, dz, db, q=q, q_exp=e), sets, n * d * (6 + 33 / 32), 0
+
+    def store(n, d):
+        sets = [(rows(n, d), *coded(n, d)) for _ in range(2)]
+        return lambda x, q, e: cu.ckpt8_store(x, d, None, n, q, e), sets, n * d * (2 + 33 / 32), 0
+
+    def load(n, d):
+        sets = [(rows(n, d), *coded(n, d)) for _ in range(2)]
+        return lambda x, q, e: cu.ckpt8_load(q, e, d, None, n, x), sets, n * d * (2 + 33 / 32), 0
+
+    def dw(n, k, m):
+        gw = torch.zeros(m, k, device=dev)
+        sets = [(rows(n, m), *coded(n, k)) for _ in range(2)]
+        return lambda dy, q, e: cu.ckpt8_dw(dy, q, e, None, n, gw, err), sets, n * (2 * m + k * 33 / 32), 2 * n * k * m
+
+    n = int(139058 * s)
+    out = []
+    for make, dims in ((norm, (n, 256)), (norm_bwd, (int(1000000 * s), 128)), (linear, (n, 256, 256)),
+                       (linear, (n, 512, 256)), (linear, (131072, 1024, 1024)), (act_bwd, (n, 256)), (store, (n, 512)),
+                       (load, (n, 512)), (dw, (int(3250 * s), 512, 256)), (dw, (int(500000 * s), 512, 256))):
+        fn, sets, moved, flops = make(*dims)
+
+        def pair():
+            fn(*sets[0])
+            fn(*sets[1])
+
+        t = _time(pair, iters=iters, warmup=5 if iters > 1 else 0) / 2
+        out.append({"bench": "residual_" + make.__name__, "dims": list(dims), "ms": t, "gb_s": moved / t / 1e6,
+                    "hbm_frac_of_measured": moved / t / 1e6 / HBM_GBS, "tflop_s": flops / t / 1e9,
+                    "bf16_frac_of_measured": flops / t / 1e9 / BF16_TFLOPS})
+    return out
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--scale", type=float, default=1.0)
-    ap.add_argument("--part", default="gemm,aggregate", help="comma list of gemm, aggregate, head, repart, ar")
+    ap.add_argument("--part", default="gemm,aggregate", help="comma list of gemm, aggregate, residual, head, repart, ar")
+    ap.add_argument("--iters", type=int, default=20, help="of the residual part")
     ap.add_argument("--ar-bytes", type=int, default=256 << 20)
     a = ap.parse_args()
     s = a.scale
@@ -293,6 +364,8 @@ def main():
     if "aggregate" in parts:
         rows += [aggregate_case(int(20853 * s), int(133975 * s), 14, 104),
                  aggregate_case(int(3250 * s), int(20853 * s), 8, 256)]
+    if "residual" in parts:
+        rows += residual_cases(s, a.iters)
     if "head" in parts:
         rows += [head_case()]
     if "repart" in parts:
