@@ -38,16 +38,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 // Bounded wait; returns false when the deadline passed or another role aborted.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  // the timer is read after the first polls only: an ordinary wait ends before
   uint64_t t0 = 0;
-  for (;;) {
-    // the timer is read after the first polls only: an ordinary wait ends before
-    for (int i = 0; i < 256; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+  uint32_t polls = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++polls & 255u) != 0) continue;
     if (*abort_flag) return false;
     const uint64_t now = globaltimer_ns();
     if (t0 == 0) t0 = now;
     if (now - t0 > kWaitNs) return false;
   }
+  return true;
 }
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
