@@ -20,8 +20,8 @@
 // which write zeros for the rows past the live ones.
 //
 // What bounds it: the bf16 form of the rows never leaves the SM; HBM sees dY once and 33/32
-// bytes a kept value.  500009 x 512 x 256 (kept columns x dY's) takes 151 us, where HBM wants
-// 81 and the products 78.  A pair spends some 1250 cycles on a block whose products take 640:
+// bytes a kept value.  500009 x 512 x 256 (kept columns x dY's) takes 141 us, where HBM wants
+// 81 and the products 78.  A pair spends some 1200 cycles on a block whose products take 640:
 // the loads alone took 103 us, and conversion, loads and the products' operand reads share
 // the SM's shared memory.
 //

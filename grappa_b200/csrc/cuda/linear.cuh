@@ -21,6 +21,13 @@
 // form is 32 accumulator registers of one thread, so its largest magnitude needs no
 // exchange.
 //
+// The tensor core adds each 16 columns of K into its fp32 accumulator by truncation: z is off by
+// up to K / 16 steps of 2^-23 of the largest partial sum, far below bf16's or a code's step,
+// but a value that close to the middle between two codes may get the other one.
+//
+// Measured: 139058 x 512 x 256 39 us (SiLU, residual and 8-bit z: 59, 85 % of the copy's
+// rate), 131072 x 1024 x 1024 195 us = 1410 TFLOP/s (258).
+//
 // Rows >= the live count are not written.  Barrier waits are bounded as in gemm.cu.
 #pragma once
 #include <algorithm>
