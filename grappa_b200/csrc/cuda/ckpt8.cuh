@@ -107,17 +107,7 @@ __device__ __forceinline__ __nv_bfloat162 group8_scale_bf16(uint32_t byte) {
   return *reinterpret_cast<const __nv_bfloat162*>(&s);
 }
 
-// Eight consecutive columns of a bf16 or fp32 row (16-byte aligned), as fp32 and back.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  if constexpr (sizeof(T) == 2) {
-    bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), v);
-  } else {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  }
-}
+// Eight consecutive columns into a bf16 or fp32 row (16-byte aligned).
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* v) {
   if constexpr (sizeof(T) == 2) {

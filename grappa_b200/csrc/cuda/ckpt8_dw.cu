@@ -460,7 +460,9 @@ DwPlan plan_for(int M, int N, int cap, int num_sms) {
   DwPlan p;
   const int64_t kb = ceil_div(std::max(cap, 1), kRows);
   p.cg = M > 128 && N > 128 && ceil_div(M, 256) * ceil_div(N, 256) * kb >= 3ll * num_sms ? 2 : 1;
-  p.cluster = p.cg == 1 && kb <= 4 * kSplitsCluster;
+  constexpr int kClusterKb = 4 * kSplitsCluster;
+  static_assert(kClusterKb <= DwSmem<1>::kChain, "a cluster's CTA has one chain");
+  p.cluster = p.cg == 1 && kb <= kClusterKb;
   p.min_kb = p.cluster ? 2 : 4;
   p.m_tiles = static_cast<int>(ceil_div(M, 128 * p.cg));
   p.n_tiles = static_cast<int>(ceil_div(N, 128 * p.cg));
