@@ -868,7 +868,8 @@ class SageEngine(BlockEngine):
                 if self.full_graph or (self.L - 2 - l) not in (getattr(self.sm, "tptr", None) or {}):
                     spec["dH"] = torch.zeros((rows, op), dtype=torch.float32, device=dev)
             else:
-                spec["ce_fused"] = op <= 64
+                # the fused epilogue counts every row; full-graph rows are selected by a mask
+                spec["ce_fused"] = op <= 64 and not self.full_graph
                 spec["head"] = (SAGE_FUSED_HEAD and l > 0 and not self.full_graph
                                 and self.cu.sage_head_supported(ip, self.n_classes))
                 # the previous layer keeps fp32 gradient rows (scatter backward): the head
@@ -1027,7 +1028,8 @@ class ResidualSageEngine(SageEngine):
             else:
                 s["X"] = torch.zeros((rows, K), **bf)
             if last:
-                s["ce_fused"] = op <= 64
+                # the fused epilogue counts every row; full-graph rows are selected by a mask
+                s["ce_fused"] = op <= 64 and not self.full_graph
                 if not s["ce_fused"]:
                     s["logits"] = torch.zeros((rows, op), **bf)
             else:
@@ -1076,7 +1078,7 @@ class ResidualSageEngine(SageEngine):
                               residual=self.lay[l - 1]["H"] if s["res"] else None, dropout_p=p,
                               counters=self.counters if p > 0 else None, salt=l, **(s["Z"] if training else {}))
             elif s["ce_fused"]:
-                labels, mask, n_sel = self._labels_rows()
+                labels, _, _ = self._labels_rows()
                 cu.gemm(s["X"], False, s["W"], False, s["rows"], self._n_dst(h), s["op"], s["K"], None, 1,
                         self._ce_dummy, GEMM_CROSS_ENTROPY, s["bias"], 0, 0.0, None, 0, labels, self.n_classes, s["dY"],
                         self.fstats[2:3], self.istats[0:1], None, self._n_dst(h), s["gb"] if training else None,
