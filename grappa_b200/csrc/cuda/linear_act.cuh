@@ -34,12 +34,15 @@ __device__ __forceinline__ F2 logistic2(F2 x) {
 // v[0], v[1] become their activations.  One reciprocal serves the pair (1 / a = b / (a b):
 // exponentials and reciprocals run at an eighth of the FMA rate and bound the epilogue of a
 // layer), so a and b stay below 2^60: z is cut off below at the point where p is 2^-60 and
-// z p is less than 1e-16 in magnitude.
+// z p is less than 1e-16 in magnitude.  The exponents take the cut-off for a NaN (fmaxf), or
+// the pair's reciprocal would carry it into the other value; the factor z keeps it.
 __device__ __forceinline__ float above(float z, float least) {  // a NaN stays
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(least));
   return r;
 }
+__device__ __forceinline__ F2 factor2(const float* v, float least) { return f2(above(v[0], least), above(v[1], least)); }
+__device__ __forceinline__ F2 argument2(const float* v, float least) { return f2(fmaxf(v[0], least), fmaxf(v[1], least)); }
 __device__ __forceinline__ void times_logistic2(F2 z, F2 x, float* v) {
   float a, b, r;
   unpack(x, a, b);
@@ -50,13 +53,14 @@ __device__ __forceinline__ void times_logistic2(F2 z, F2 x, float* v) {
   unpack(mul2(z, f2(b * r, a * r)), v[0], v[1]);
 }
 __device__ __forceinline__ void silu2(float* v) {
-  const F2 z = f2(above(v[0], -41.5f), above(v[1], -41.5f));
-  times_logistic2(z, mul2(z, both(-kLog2e)), v);
+  constexpr float kLeast = -41.5f;
+  times_logistic2(factor2(v, kLeast), mul2(argument2(v, kLeast), both(-kLog2e)), v);
 }
 __device__ __forceinline__ void gelu2(float* v) {
-  const F2 z = f2(above(v[0], -7.4f), above(v[1], -7.4f));
+  constexpr float kLeast = -7.4f;
+  const F2 z = argument2(v, kLeast);
   const F2 u = fma2(mul2(z, z), both(-kGelu2C3 * kLog2e), both(-kGelu2C * kLog2e));
-  times_logistic2(z, mul2(z, u), v);
+  times_logistic2(factor2(v, kLeast), mul2(z, u), v);
 }
 
 // g[0], g[1] times the slopes at z[0], z[1].  p (1 - p) is 0 for large |z|, where the other
