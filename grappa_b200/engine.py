@@ -32,11 +32,10 @@ import math
 import os
 
 import torch
-import torch.nn.functional as F
 
 from grappa_b200 import _native
+from grappa_b200.models import model_activation
 from grappa_b200.models.flat import pad8
-from grappa_b200.ops import ref
 from grappa_b200.sampler_gpu import C_EPOCH, C_STEP, GpuNeighborSampler, new_counters
 
 GEMM_STORE_BF16, GEMM_STORE_F32, GEMM_ATOMIC_F32, GEMM_CROSS_ENTROPY = 0, 1, 2, 3
@@ -289,18 +288,29 @@ class GpuWalkSampler(GpuNeighborSampler):
 
 
 # ---------------------------------------------------------------------- engines
+def checked_activation(model, known):
+    """The name of the model's activation, which has to be one of ``known``."""
+    act = model_activation(model)
+    if act not in known:
+        raise ValueError(f"the kernels of {model.name} have the activations {', '.join(known)} (gelu in its tanh form); "
+                         f"the model's is {act or 'another function'}")
+    return act
+
+
 class BlockEngine:
     """Shared parts: parameters (flat fp32 master, bf16 working copy, gradient, Adam
     moments), device counters, the block source, the optimizer step, CUDA-graph
     capture.  Subclasses implement ``_alloc_layers``, ``_forward`` and ``_backward``."""
 
     model_name = None
+    activations = ("relu",)  # that the layers' kernels apply (names of models.ACTIVATIONS)
 
     def __init__(self, model, n_nodes_cap, fanouts, batch_size, device, lr=3e-3, comm=None, seed=0,
                  fused_allreduce=True, use_cuda_graph=True, betas=(0.9, 0.999), eps=1e-8, blocks=None,
                  overlap_sampling=True, overlap_allreduce=True, ar_mode=None):
         if getattr(model, "name", None) != self.model_name:
             raise ValueError(f"{type(self).__name__} trains {self.model_name} models")
+        self.activation = checked_activation(model, self.activations)
         self.cu = LaunchCounter(_native.cuda())
         self.launches_per_step = 0
         self.model = model
@@ -959,14 +969,13 @@ class SageEngine(BlockEngine):
                    prev["rows"])
 
 
-#: activation functions of the linear kernel's epilogue
-LINEAR_ACTS = {F.relu: 1, ref.gelu: 2, F.silu: 3}
+#: activations of the linear kernel's epilogue
+LINEAR_ACTS = {"relu": 1, "gelu": 2, "silu": 3}
 
 
 def needs_residual_engine(model):
     """Whether a GraphSAGE model uses what only the residual layers' kernels have."""
-    return bool(model.norm is not None or model.residual
-                or (model.activation is not F.relu and model.activation in LINEAR_ACTS))
+    return bool(getattr(model, "norm", None) is not None or model_activation(model) in ("gelu", "silu"))
 
 
 class ResidualSageEngine(SageEngine):
@@ -981,6 +990,8 @@ class ResidualSageEngine(SageEngine):
     layers share: per hidden layer of width d, 4d + groups bytes a row instead of 8d.
     The gradient of the residual stream is fp32 and passes through the norms' backward."""
 
+    activations = tuple(LINEAR_ACTS)
+
     def __init__(self, *args, act_bits=16, **kw):
         if act_bits not in (8, 16):
             raise ValueError("act_bits must be 8 or 16")
@@ -994,9 +1005,7 @@ class ResidualSageEngine(SageEngine):
         dev, m, eight = self.device, self.model, self.act_bits == 8
         bf = dict(dtype=torch.bfloat16, device=dev)
         f32 = dict(dtype=torch.float32, device=dev)
-        if m.activation not in LINEAR_ACTS:
-            raise ValueError("the GPU engine has ReLU, GELU (tanh form) and SiLU")
-        self.act = LINEAR_ACTS[m.activation]
+        self.act = LINEAR_ACTS[self.activation]
 
         def codes(rows, dim):
             w = (dim + 31) // 32 * 32

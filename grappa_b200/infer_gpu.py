@@ -12,8 +12,9 @@ its running statistics, on buffers sized for the block.
 import torch
 
 from grappa_b200 import _native
-from grappa_b200.engine import (AGG_GCN, AGG_MEAN, AGG_SUM, AGG_WEIGHTED, GEMM_STORE_BF16, LINEAR_ACTS, gemm_bn,
-                                needs_residual_engine)
+from grappa_b200.engine import (AGG_GCN, AGG_MEAN, AGG_SUM, AGG_WEIGHTED, GEMM_STORE_BF16, LINEAR_ACTS, checked_activation,
+                                gemm_bn, needs_residual_engine)
+from grappa_b200.models import model_activation
 from grappa_b200.models.flat import pad8
 
 
@@ -75,7 +76,7 @@ def _sage(ctx, model, l, last, ip_, ix, n_dst, n_src, x):
         cu.aggregate(ip_, ix, None, n_dst, R, n, None, ip, AGG_MEAN, None, None, None, X, ip, 0, 0.0, 0, ctx.err)
         H = ctx.zeros(R, op)
         cu.linear_fwd(X, ctx.seg(layer.seg_w), ctx.count(n_dst), R, H, ctx.err, bias=ctx.seg(layer.seg_b, False)[0],
-                      act=0 if last else LINEAR_ACTS[model.activation],
+                      act=0 if last else LINEAR_ACTS[model_activation(model)],
                       residual=x if model.has_residual(l) else None)
         return H[:n_dst, :layer.out_feats]
     cu.aggregate(ip_, ix, None, n_dst, R, x, None, ip, AGG_MEAN, None, None, None, X, ip, 0, 0.0, 0, ctx.err)
@@ -177,11 +178,13 @@ def infer_layer(model, layer_i, block, h):
     dev = h.device
     if dev.type != "cuda":
         raise ValueError("infer_layer runs on CUDA tensors")
+    last = layer_i == len(model.layers) - 1
+    if not last or model.name == "pinsage":
+        checked_activation(model, tuple(LINEAR_ACTS) if model.name == "sage" else ("relu",))
     ctx = _Ctx(model, dev)
     n_dst, n_src = block.num_dst_nodes(), block.num_src_nodes()
     ip_ = block.indptr.to(dev, torch.int32).contiguous()
     ix = block.indices.to(dev, torch.int32).contiguous()
-    last = layer_i == len(model.layers) - 1
     layer = model.layers[layer_i]
     name = model.name
     if name == "sage":

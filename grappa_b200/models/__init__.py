@@ -15,10 +15,45 @@ from grappa_b200.models.flat import FlatModule, pad8
 from grappa_b200.models.layers import GATConv, GINConv, GINMLP, GraphConv, RMSNorm, SAGEConv, WeightedSAGEConv
 from grappa_b200.ops import ref
 
-__all__ = ["SAGE", "GCN", "GAT", "GIN", "PinSAGE", "get_model", "ACTIVATIONS"]
+__all__ = ["SAGE", "GCN", "GAT", "GIN", "PinSAGE", "get_model", "ACTIVATIONS", "activation_name", "model_activation"]
 
 #: activations by name; the GPU engine knows these functions
 ACTIVATIONS = {"relu": F.relu, "gelu": ref.gelu, "silu": F.silu}
+
+
+def activation_name(fn):
+    """The name in ``ACTIVATIONS`` of the function that ``fn`` computes, or None.  A module, a
+    lambda or another spelling (torch.relu, nn.SiLU()) is known by its values, in 64 bits, at
+    points around zero and far from it; GELU's two forms differ there by up to 5e-4.  A module
+    with parameters is none of them: it may become another function in training."""
+    for name, known in ACTIVATIONS.items():
+        if fn is known:
+            return name
+    if isinstance(fn, nn.Module) and next(fn.parameters(), None) is not None:
+        return None
+    far = torch.tensor([10.0, 30.0, 1e3, 1e5], dtype=torch.float64)
+    x = torch.cat([torch.linspace(-8, 8, 161, dtype=torch.float64), far, -far])
+    try:
+        with torch.no_grad():
+            y = fn(x.clone())
+            for name, known in ACTIVATIONS.items():
+                if torch.allclose(y, known(x), rtol=1e-9, atol=1e-12):
+                    return name
+    except Exception:
+        pass  # not a function of a 64-bit CPU tensor: unknown
+    return None
+
+
+def model_activation(model):
+    """``activation_name`` of the activation that a model applies between its layers (PinSAGE: in
+    each); models without a choice have ReLU."""
+    if getattr(model, "name", None) == "pinsage":
+        fn = model.layers[0].act
+    elif len(model.layers) == 1:
+        return "relu"  # applied nowhere
+    else:
+        fn = getattr(model, "activation", None)
+    return "relu" if fn is None else activation_name(fn)
 
 
 class _Base(FlatModule):
