@@ -54,7 +54,7 @@ def apply_layer(model, layer_i, block, h):
         h = layer(block, (h, h_dst))
         return h.mean(1) if last else model.activation(h.flatten(1))
     if model.name == "sage":
-        return model.run_layer(layer_i, block, h)
+        return model.run_layer(layer_i, block, h, dropout=False)
     if model.name == "gcn":
         h = layer(block, h)
         return h if last else model.activation(h)

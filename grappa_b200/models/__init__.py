@@ -122,13 +122,15 @@ class SAGE(_Base):
         layer = self.layers[l]
         return self.residual and 0 < l < self.n_layers - 1 and layer.in_feats == layer.out_feats
 
-    def run_layer(self, l, block, h):
-        """Layer l with its norm, activation, dropout and residual."""
+    def run_layer(self, l, block, h, dropout=True):
+        """Layer l with its norm, activation, dropout (in training) and residual."""
         n = self.norms[l - 1](h) if self.norm is not None and l > 0 else h
         z = self.layers[l](block, n)
         if l == self.n_layers - 1:
             return z
-        z = self._drop(self.activation(z), l, pad8(self.layers[l].out_feats))
+        z = self.activation(z)
+        if dropout:
+            z = self._drop(z, l, pad8(self.layers[l].out_feats))
         return h[: block.num_dst_nodes()] + z if self.has_residual(l) else z
 
     def forward(self, blocks, x):
