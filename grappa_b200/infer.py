@@ -53,10 +53,10 @@ def apply_layer(model, layer_i, block, h):
     if model.name == "gat":
         h = layer(block, (h, h_dst))
         return h.mean(1) if last else model.activation(h.flatten(1))
-    if model.name == "sage":
+    if model.name == "sage" and getattr(model, "norm", None) is not None:
         return model.run_layer(layer_i, block, h, dropout=False)
-    if model.name == "gcn":
-        h = layer(block, h)
+    if model.name in ("sage", "gcn"):
+        h = layer(block, (h, h_dst)) if model.name == "sage" else layer(block, h)
         return h if last else model.activation(h)
     if model.name == "gin":
         h = layer(block, (h, h_dst))

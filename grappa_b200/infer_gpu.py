@@ -67,8 +67,8 @@ def _sage(ctx, model, l, last, ip_, ix, n_dst, n_src, x):
     R = _rows(n_dst)
     X = ctx.zeros(R, 2 * ip)
     if needs_residual_engine(model):
-        n = x
-        if model.norm is not None and l > 0:
+        n, norms = x, getattr(model, "norm", None) is not None
+        if norms and l > 0:
             n = torch.zeros_like(x)
             norm = model.norms[l - 1]
             cu.rmsnorm_fwd(x, norm.dim, ctx.count(n_src), x.shape[0], ctx.seg(norm.seg, False)[0], norm.eps, n,
@@ -77,7 +77,7 @@ def _sage(ctx, model, l, last, ip_, ix, n_dst, n_src, x):
         H = ctx.zeros(R, op)
         cu.linear_fwd(X, ctx.seg(layer.seg_w), ctx.count(n_dst), R, H, ctx.err, bias=ctx.seg(layer.seg_b, False)[0],
                       act=0 if last else LINEAR_ACTS[model_activation(model)],
-                      residual=x if model.has_residual(l) else None)
+                      residual=x if norms and model.has_residual(l) else None)
         return H[:n_dst, :layer.out_feats]
     cu.aggregate(ip_, ix, None, n_dst, R, x, None, ip, AGG_MEAN, None, None, None, X, ip, 0, 0.0, 0, ctx.err)
     H = ctx.zeros(R, op)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 import torch.nn.functional as F
+from torch import nn
 
 from grappa_b200.block import Block
 from grappa_b200.infer import apply_layer
@@ -30,3 +31,19 @@ def test_layer_inference_draws_no_dropout(kw):
     for l in range(4):
         h = apply_layer(m, l, b, h).detach()
         assert torch.equal(h, want[l])
+
+
+def test_layer_inference_of_a_users_own_sage():
+    """A module of the same name that has layers and an activation, and nothing else."""
+    class Own(nn.Module):
+        name = "sage"
+
+        def __init__(self, of):
+            super().__init__()
+            self.layers, self.activation = of.layers, of.activation
+
+    m = SAGE(8, 16, 4, 2, F.relu, 0.0)
+    b, x = block(), torch.randn(30, 8)
+    own = Own(m)
+    h = apply_layer(own, 0, b, x)
+    torch.testing.assert_close(apply_layer(own, 1, b, h), m([b, b], x))
