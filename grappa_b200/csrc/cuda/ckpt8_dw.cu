@@ -159,6 +159,11 @@ __global__ void __launch_bounds__(DwSmem<CG>::kThreads, 1)
   // number of the partly filled block (-1: none here)
   const int tail = n % kRows != 0 && nkb > 0 && row0(nkb - 1) + kRows > n ? nkb - 1 : -1;
   float* part = a.work + static_cast<int64_t>(blockIdx.x) * (128 * NT);
+  // a wait for arrivals of both CTAs
+  auto wait_both = [&](uint64_t* bar, uint32_t parity) {
+    if constexpr (CG == 2) return mbar_wait_cluster(bar, parity, &abort_flag);
+    return mbar_wait_all(bar, parity, &abort_flag);
+  };
   // waits until the products of block j are done (j in order for every caller,
   // or after a later block: a wait by parity must not begin two phases early)
   auto products_done = [&](int j) { return mbar_wait_all(&done_bar[j % kDone], (j / kDone) & 1u, &abort_flag); };
@@ -205,9 +210,9 @@ __global__ void __launch_bounds__(DwSmem<CG>::kThreads, 1)
         const int s = i % kYSlots, b = i % kBSlots;
         const int chain = i / kChain, ab = chain & 1;
         const bool first = i % kChain == 0;
-        if ((first && chain >= 2 && !mbar_wait_all(&acc_empty[ab], ((chain >> 1) - 1) & 1u, &abort_flag)) ||
+        if ((first && chain >= 2 && !wait_both(&acc_empty[ab], ((chain >> 1) - 1) & 1u)) ||
             !mbar_wait_all(&y_full[s], (i / kYSlots) & 1u, &abort_flag) ||
-            !mbar_wait_all(&b_full[b], (i / kBSlots) & 1u, &abort_flag)) {
+            !wait_both(&b_full[b], (i / kBSlots) & 1u)) {
           if (lane == 0) set_error(a.err, kErrMmaTimeout);
           abort_flag = 1;
           break;

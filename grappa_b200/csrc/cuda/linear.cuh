@@ -195,7 +195,9 @@ __global__ void __launch_bounds__(LSmem<BN, CG, true, true>::kThreads, LSmem<BN,
       bool stop = false;
       for (int64_t t = first; t < tiles && !stop; t += step, ++lt) {
         const int b = lt & 1;
-        if (lt >= 2 && !mbar_wait_all(&acc_empty[b], ((lt >> 1) - 1) & 1u, &abort_flag)) {
+        const uint32_t last = ((lt >> 1) - 1) & 1u;
+        if (lt >= 2 && !(CG == 2 ? mbar_wait_cluster(&acc_empty[b], last, &abort_flag)
+                                 : mbar_wait_all(&acc_empty[b], last, &abort_flag))) {
           if (lane == 0) set_error(a.err, kErrMmaTimeout);
           abort_flag = 1;
           break;

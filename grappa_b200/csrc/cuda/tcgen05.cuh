@@ -25,15 +25,27 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
                : "memory");
 }
+// CLUSTER: a poll that may observe the other CTA's arrivals, without ordering anything (the
+// fence of mbar_wait_cluster does)
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
   return ok != 0;
 }
 // Bounded wait; returns false when the deadline passed or another role aborted.
@@ -67,12 +79,13 @@ __device__ __forceinline__ bool elect_one() {
 }
 // mbar_wait by a converged warp, with the same answer in every lane.  A vote a poll keeps the
 // warp converged (lanes that leave the loop by themselves cost 1 to 3 % of the kernels here).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   constexpr uint32_t kAll = 0xffffffffu;
-  if (__all_sync(kAll, mbar_try_wait(bar, parity))) return true;
+  if (__all_sync(kAll, mbar_try_wait<CLUSTER>(bar, parity))) return true;
   uint64_t t0 = 0;
   uint32_t polls = 0;
-  while (!__all_sync(kAll, mbar_try_wait(bar, parity))) {
+  while (!__all_sync(kAll, mbar_try_wait<CLUSTER>(bar, parity))) {
     if ((++polls & 255u) != 0) continue;
     if (__any_sync(kAll, *abort_flag)) return false;
     const uint64_t now = globaltimer_ns();
@@ -198,14 +211,21 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
       "h"(static_cast<uint16_t>(3))
       : "memory");
 }
-// Arrives on a barrier of the other (or this) CTA of the cluster.  What it hands over is
-// tensor memory that has been read (tcgen05.wait::ld and the fence before it) or shared
-// memory written through fence.proxy.async, so the default scope is enough on both sides;
-// with .release.cluster here and .acquire.cluster on the wait, every hand-over also waited
-// for the warp's global stores (linear 139058 x 512 x 256 with GELU and 8-bit z: 57.9 us
-// instead of 51.9).
+// Arrives on a barrier of the other (or this) CTA of the cluster, and the wait for such
+// arrivals.  They hand over shared memory that this CTA's threads wrote (after fence.proxy.async)
+// or tensor memory that they read (after tcgen05.wait::ld and its fence) to products issued by
+// the other CTA: ordered at cluster scope, for shared memory alone.  A release of all memory
+// (.release.cluster on the arrival) also waited for the warp's global accesses: weight gradient
+// 500009 x 512 x 256 192 us instead of 141, linear 139058 x 512 x 256 with GELU and 8-bit z 57.9
+// instead of 51.9.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (!mbar_wait_all<true>(bar, parity, abort_flag)) return false;
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+  return true;
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
