@@ -78,6 +78,17 @@ struct DwPlan {
   bool cluster;          // a tile's splits are one cluster that sums its partial tiles itself
 };
 
+// The first `cols` of eight columns at p, zeros after them.  A row may end with its M columns,
+// so a piece that is not whole is read column by column.
+__device__ __forceinline__ uint4 row_piece(const __nv_bfloat16* p, int cols) {
+  if (cols >= 8) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (j < cols) w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[j]) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Four sums into row m, columns nn .. nn + 3 of gW.
 __device__ __forceinline__ void add_quad(const Ckpt8DwArgs& a, int m, int nn, float4 s) {
   if (m >= a.M || nn >= a.N) return;
@@ -313,7 +324,7 @@ __global__ void __launch_bounds__(DwSmem<CG>::kThreads, 1)
 #pragma unroll 1
         for (int p = 0; p < 8; ++p) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (r0 + k < n && 8 * p < cols) v = first_columns(*reinterpret_cast<const uint4*>(y + 8 * p), cols - 8 * p);
+          if (r0 + k < n && 8 * p < cols) v = row_piece(y + 8 * p, cols - 8 * p);
           *reinterpret_cast<uint4*>(sy + ((p ^ (k & 7)) << 4)) = v;
         }
       }

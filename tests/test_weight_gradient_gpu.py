@@ -57,3 +57,32 @@ def test_pairs_repeat_bit_for_bit_over_other_data(n, k, m):
                 first[i] = gw
             assert torch.equal(gw, first[i])
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("m", [1, 3, 5, 65, 130, 255])
+@pytest.mark.parametrize("n,cap,k", [(1, 1, 40), (37, 37, 64), (2001, 2001, 136), (60063, 60063, 200)])
+def test_rows_that_end_with_their_storage(n, cap, k, m):
+    """The last row of dY ends where its storage ends, without columns to a multiple of 8."""
+    g = gen_for("end", n, k, m)
+    ld = (m + 7) // 8 * 8
+    store = torch.randn((n - 1) * ld + m, generator=g, device=DEV).to(BF)
+    dy = store.as_strided((n, m), (ld, 1))
+    q, e, x = coded(g, n, k)
+    gw = torch.full((m, k), float("nan"), device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cu().ckpt8_dw(dy, q, e, None, cap, gw, err, accumulate=False)
+    want, size = dy.double().t() @ x, dy.double().abs().t() @ x.abs()
+    assert bool(((gw.double() - want).abs() <= tolerance(n, size)).all()) and int(err) == 0
+
+
+def test_columns_past_m_do_not_count():
+    """A NaN right behind the M columns, in the row that is read in parts and in the others."""
+    g = gen_for("behind")
+    n, k, m = 133, 96, 45
+    dy = torch.full((n, 64), float("nan"), dtype=BF, device=DEV)
+    dy[:, :m] = torch.randn((n, m), generator=g, device=DEV).to(BF)
+    q, e, x = coded(g, n, k)
+    gw = torch.zeros((m, k), device=DEV)
+    cu().ckpt8_dw(dy, q, e, None, n, gw, torch.zeros(1, dtype=torch.int32, device=DEV), accumulate=False)
+    want, size = dy[:, :m].double().t() @ x, dy[:, :m].double().abs().t() @ x.abs()
+    assert bool(((gw.double() - want).abs() <= tolerance(n, size)).all())
