@@ -1030,7 +1030,7 @@ class ResidualSageEngine(SageEngine):
             s = dict(h=h, ip=ip, op=op, K=K, rows=rows, srows=srows, last=last, res=m.has_residual(l),
                      W=self._seg(layer.seg_w, self.wbf), bias=self._seg(layer.seg_b)[0],
                      gW=self._seg(layer.seg_w, self.grad), gb=self._seg(layer.seg_b, self.grad)[0])
-            lazy.append((s, "dY", scratch(f"dY{l & 1}", rows, op, torch.bfloat16)))
+            lazy.append((s, "dY", scratch("dY", rows, op, torch.bfloat16)))
             if eight:
                 lazy.append((s, "X", scratch("X", rows, K, torch.bfloat16)))
                 s["Xq"] = codes(rows, K)
@@ -1113,7 +1113,8 @@ class ResidualSageEngine(SageEngine):
         h = s["h"]
         n = self._n_dst(h)
         if not s["last"]:
-            # dY of this parity is read by layer l + 2's weight gradient on the auxiliary stream
+            # the layers share dY: the weight gradient of the layer above, on the auxiliary stream,
+            # has to have read it
             self._join_aux()
             cu.linear_act_bwd(s["dH"], self.model.layers[l].out_feats, n, s["rows"], self.act, s["dY"], s["gb"],
                               clear_dout="norm" not in s and self.model.norm is None, dropout_p=self.p,
