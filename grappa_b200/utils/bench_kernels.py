@@ -35,6 +35,43 @@ def _time(fn, iters=50, warmup=5):
     return a.elapsed_time(b) / iters
 
 
+def _under_load(fn, seconds=1.0):
+    """ms a call over ``seconds`` of calls back to back, with the SM clock that was sampled
+    meanwhile and the reasons that held it down (read through NVML, nothing is set)."""
+    import threading
+    import time
+
+    import pynvml
+
+    pynvml.nvmlInit()
+    uuid = "GPU-" + str(torch.cuda.get_device_properties(0).uuid)
+    h = pynvml.nvmlDeviceGetHandleByUUID(uuid)
+    mhz, bits, stop = [], 0, threading.Event()
+
+    def sample():
+        nonlocal bits
+        while not stop.wait(0.02):
+            mhz.append(pynvml.nvmlDeviceGetClockInfo(h, pynvml.NVML_CLOCK_SM))
+            bits |= pynvml.nvmlDeviceGetCurrentClocksEventReasons(h)
+
+    calls = max(10, int(seconds / max(_time(fn, 10) * 1e-3, 1e-6)))
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t = threading.Thread(target=sample)
+    t.start()
+    a.record()
+    for i in range(calls):
+        fn()
+        if i % 200 == 199:
+            time.sleep(0)
+    b.record()
+    torch.cuda.synchronize()
+    stop.set()
+    t.join()
+    pynvml.nvmlShutdown()
+    names = {0x4: "sw_power_cap", 0x8: "hw_slowdown", 0x20: "sw_thermal_slowdown", 0x40: "hw_thermal_slowdown"}
+    return a.elapsed_time(b) / calls, sorted(mhz)[len(mhz) // 2], [v for k, v in names.items() if bits & k]
+
+
 def gemm_case(M, K, N, bn=None, p=0.0):
     from grappa_b200.engine import gemm_bn
 
@@ -275,10 +312,11 @@ def repart_case(n_part=600_000, deg=50, n_global=2_449_029, halo=400_000, dim=10
     return res
 
 
-def residual_cases(s=1.0, iters=20):
+def residual_cases(s=1.0, iters=20, only="", clocks=False):
     """The residual layer's operators, two sets of buffers in turn (together larger than L2
     but for the small ones): time, bytes that have to move and products.  iters=1 runs each
-    once, without warm-up (for a profiler)."""
+    once, without warm-up (for a profiler); ``only`` takes the cases of one name; ``clocks``
+    adds the time of a call and the SM clock over a second of calls."""
     cu = _native.cuda()
     dev = torch.device("cuda", 0)
     bf, f32 = torch.bfloat16, torch.float32
@@ -330,8 +368,10 @@ def residual_cases(s=1.0, iters=20):
     n = int(139058 * s)
     out = []
     for make, dims in ((norm, (n, 256)), (norm_bwd, (int(1000000 * s), 128)), (linear, (n, 256, 256)),
-                       (linear, (n, 512, 256)), (linear, (131072, 1024, 1024)), (act_bwd, (n, 256)), (store, (n, 512)),
+                       (linear, (n, 512, 256)), (linear, (int(131072 * s), 1024, 1024)), (act_bwd, (n, 256)), (store, (n, 512)),
                        (load, (n, 512)), (dw, (int(3250 * s), 512, 256)), (dw, (int(500000 * s), 512, 256))):
+        if only and make.__name__ != only:
+            continue
         fn, sets, moved, flops = make(*dims)
 
         def pair():
@@ -342,6 +382,9 @@ def residual_cases(s=1.0, iters=20):
         out.append({"bench": "residual_" + make.__name__, "dims": list(dims), "ms": t, "gb_s": moved / t / 1e6,
                     "hbm_frac_of_measured": moved / t / 1e6 / HBM_GBS, "tflop_s": flops / t / 1e9,
                     "bf16_frac_of_measured": flops / t / 1e9 / BF16_TFLOPS})
+        if clocks:
+            held, mhz, reasons = _under_load(pair)
+            out[-1].update(ms_for_a_second=held / 2, sm_mhz=mhz, reasons=reasons)
     return out
 
 
@@ -350,6 +393,8 @@ def main():
     ap.add_argument("--scale", type=float, default=1.0)
     ap.add_argument("--part", default="gemm,aggregate", help="comma list of gemm, aggregate, residual, head, repart, ar")
     ap.add_argument("--iters", type=int, default=20, help="of the residual part")
+    ap.add_argument("--only", default="", help="one case of the residual part: norm, norm_bwd, linear, act_bwd, store, load, dw")
+    ap.add_argument("--clocks", action="store_true", help="sample the SM clock over a second of each case of the residual part")
     ap.add_argument("--ar-bytes", type=int, default=256 << 20)
     a = ap.parse_args()
     s = a.scale
@@ -365,7 +410,7 @@ def main():
         rows += [aggregate_case(int(20853 * s), int(133975 * s), 14, 104),
                  aggregate_case(int(3250 * s), int(20853 * s), 8, 256)]
     if "residual" in parts:
-        rows += residual_cases(s, a.iters)
+        rows += residual_cases(s, a.iters, a.only, a.clocks)
     if "head" in parts:
         rows += [head_case()]
     if "repart" in parts:
