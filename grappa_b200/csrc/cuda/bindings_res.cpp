@@ -466,9 +466,12 @@ every run.)");
 A [>= cap, K] and W [N, K] bf16, bias [N] float32, out and residual bf16 rows of N columns
 (padded to 8; out may be the residual itself).  act: 0 none, 1 ReLU, 2 GELU (tanh form),
 3 SiLU.  The pre-activation is kept for linear_act_bwd as bf16 rows (z) and / or in 8 bits
-(q / q_exp; with ReLU a positive value keeps a code of at least 1).  Dropout draws the
-Philox mask of element r * out.stride(0) + c, as gemm does.  Rows past n = min(*n_dev, cap)
-are left as they were.  err: the engine's error word.)");
+(q / q_exp; with ReLU a positive value keeps a code of at least 1).  z is summed in fp32 by the
+tensor core, which truncates: it is short by about 8e-10 K of itself (1e-6 at K = 1024), so that
+a value that close to the middle between two codes may get the other one (3 of 100000 there);
+both stand for it equally well.  Same bits on every run.  Dropout draws the Philox mask of
+element r * out.stride(0) + c, as gemm does.  Rows past n = min(*n_dev, cap) are left as they
+were.  err: the engine's error word.)");
   m.def("linear_act_bwd", &linear_act_bwd, py::arg("dout"), py::arg("dim"), py::arg("n_dev"), py::arg("cap"),
         py::arg("act"), py::arg("dz"), py::arg("dbias") = none, py::arg("z") = none, py::arg("q") = none,
         py::arg("q_exp") = none, py::arg("clear_dout") = false, py::arg("dropout_p") = 0.0, py::arg("counters") = none,
