@@ -1,5 +1,5 @@
 // Pairs of fp32 values: one instruction for two operations (the epilogues and the
-// activation backward are bound by instruction issue before they are by HBM).
+// activation backward issue half as many).
 #pragma once
 #include <cuda_runtime.h>
 

@@ -10,6 +10,7 @@ Prints one JSON line per measurement.
 import argparse
 import json
 import math
+import time
 
 import torch
 
@@ -39,7 +40,6 @@ def _under_load(fn, seconds=1.0):
     """ms a call over ``seconds`` of calls back to back, with the SM clock that was sampled
     meanwhile and the reasons that held it down (read through NVML, nothing is set)."""
     import threading
-    import time
 
     import pynvml
 
@@ -316,11 +316,13 @@ def residual_cases(s=1.0, iters=20, only="", clocks=False):
     """The residual layer's operators, two sets of buffers in turn (together larger than L2
     but for the small ones): time, bytes that have to move and products.  iters=1 runs each
     once, without warm-up (for a profiler); ``only`` takes the cases of one name; ``clocks``
-    adds the time of a call and the SM clock over a second of calls."""
+    lets the GPU rest before each case and adds the time of a call and the SM clock over a
+    second of calls, where the power cap shows."""
     cu = _native.cuda()
     dev = torch.device("cuda", 0)
     bf, f32 = torch.bfloat16, torch.float32
     err = torch.zeros(1, dtype=torch.int32, device=dev)
+    ctr = torch.zeros(6, dtype=torch.int64, device=dev)
 
     def rows(n, d, t=bf):
         return torch.randn(n, d, device=dev).to(t)
@@ -347,6 +349,30 @@ def residual_cases(s=1.0, iters=20, only="", clocks=False):
         return lambda x, res, out, q, e: cu.linear_fwd(x, w, None, n, out, err, bias=b, act=3, residual=res, q=q,
                                                        q_exp=e), sets, n * (2 * k + 4 * m + m * 33 / 32), 2 * n * k * m
 
+    # what training with dropout, and with z in bf16, launches
+    def linear_drop(n, k, m, z16=False):
+        w, b = (rows(m, k, f32) / math.sqrt(k)).to(bf), torch.zeros(m, device=dev)
+        sets = [(rows(n, k), rows(n, m), rows(n, m), *((rows(n, m), None) if z16 else coded(n, m))) for _ in range(2)]
+        return lambda x, res, out, q, e: cu.linear_fwd(
+            x, w, None, n, out, err, bias=b, act=3, residual=res, dropout_p=0.5, counters=ctr,
+            **(dict(z=q) if z16 else dict(q=q, q_exp=e))), sets, n * (2 * k + 4 * m + m * (2 if z16 else 33 / 32)), 2 * n * k * m
+
+    def linear_drop_z16(n, k, m):
+        return linear_drop(n, k, m, True)
+
+    def act_bwd_drop(n, d):
+        db = torch.zeros(d, device=dev)
+        sets = [(rows(n, d, f32), rows(n, d), *coded(n, d)) for _ in range(2)]
+        return lambda g, dz, q, e: cu.linear_act_bwd(g, d, None, n, 2, dz, db, q=q, q_exp=e, dropout_p=0.5,
+                                                     counters=ctr), sets, n * d * (6 + 33 / 32), 0
+
+    # the norm's backward as an engine with 8-bit rows calls it: fp32 gradients, dy cleared
+    def norm_bwd_f32(n, d):
+        g, r, dg = torch.ones(d, device=dev), torch.ones(n, device=dev), torch.zeros(d, device=dev)
+        sets = [(rows(n, d, f32), *coded(n, d), rows(n, d, f32), rows(n, d, f32)) for _ in range(2)]
+        return lambda dy, q, e, dr, dx: cu.rmsnorm_bwd(dy, None, r, g, d, None, n, dx, dg, dres=dr, clear_dy=True, q=q,
+                                                       q_exp=e), sets, n * d * (16 + 33 / 32), 0
+
     def act_bwd(n, d):
         db = torch.zeros(d, device=dev)
         sets = [(rows(n, d, f32), rows(n, d), *coded(n, d)) for _ in range(2)]
@@ -369,7 +395,10 @@ def residual_cases(s=1.0, iters=20, only="", clocks=False):
     out = []
     for make, dims in ((norm, (n, 256)), (norm_bwd, (int(1000000 * s), 128)), (linear, (n, 256, 256)),
                        (linear, (n, 512, 256)), (linear, (int(131072 * s), 1024, 1024)), (act_bwd, (n, 256)), (store, (n, 512)),
-                       (load, (n, 512)), (dw, (int(3250 * s), 512, 256)), (dw, (int(500000 * s), 512, 256))):
+                       (load, (n, 512)), (dw, (int(3250 * s), 512, 256)), (dw, (int(500000 * s), 512, 256)),
+                       (linear_drop, (n, 208, 256)), (linear_drop, (n, 512, 256)), (linear_drop_z16, (n, 208, 256)),
+                       (linear_drop_z16, (n, 512, 256)), (act_bwd_drop, (n, 256)),
+                       (norm_bwd_f32, (int(1000000 * s), 128))):
         if only and make.__name__ != only:
             continue
         fn, sets, moved, flops = make(*dims)
@@ -378,6 +407,9 @@ def residual_cases(s=1.0, iters=20, only="", clocks=False):
             fn(*sets[0])
             fn(*sets[1])
 
+        if clocks:  # the short run at the clock of a GPU that has rested
+            torch.cuda.synchronize()
+            time.sleep(2.0)
         t = _time(pair, iters=iters, warmup=5 if iters > 1 else 0) / 2
         out.append({"bench": "residual_" + make.__name__, "dims": list(dims), "ms": t, "gb_s": moved / t / 1e6,
                     "hbm_frac_of_measured": moved / t / 1e6 / HBM_GBS, "tflop_s": flops / t / 1e9,
@@ -393,7 +425,9 @@ def main():
     ap.add_argument("--scale", type=float, default=1.0)
     ap.add_argument("--part", default="gemm,aggregate", help="comma list of gemm, aggregate, residual, head, repart, ar")
     ap.add_argument("--iters", type=int, default=20, help="of the residual part")
-    ap.add_argument("--only", default="", help="one case of the residual part: norm, norm_bwd, linear, act_bwd, store, load, dw")
+    ap.add_argument("--only", default="",
+                    help="the residual part's cases of one name: norm, norm_bwd, norm_bwd_f32, linear, linear_drop, "
+                         "linear_drop_z16, act_bwd, act_bwd_drop, store, load, dw")
     ap.add_argument("--clocks", action="store_true", help="sample the SM clock over a second of each case of the residual part")
     ap.add_argument("--ar-bytes", type=int, default=256 << 20)
     a = ap.parse_args()
