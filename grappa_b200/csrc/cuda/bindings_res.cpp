@@ -117,6 +117,17 @@ void all_apart(const Mat& out, const std::vector<Mat>& others) {
   for (const Mat& o : others) apart(out, o);
 }
 
+// A vector argument as a matrix of one row, for the overlap checks.
+Mat line(float* p, int64_t n, const char* name) {
+  Mat m;
+  m.p = reinterpret_cast<char*>(p);
+  m.rows = 1;
+  m.cols = m.ld = n;
+  m.es = sizeof(float);
+  m.name = name;
+  return m;
+}
+
 int32_t rows_cap(int64_t cap) {
   TORCH_CHECK(cap >= 0 && cap <= std::numeric_limits<int32_t>::max() - 256, "cap must be in [0, 2^31 - 256)");
   return static_cast<int32_t>(cap);
@@ -160,7 +171,8 @@ void rmsnorm_fwd(Tensor x, int64_t dim, OptT n_dev, int64_t cap, Tensor gamma, d
   const int64_t w = up(dim, 8);
   const Mat mx = mat(x, "x", {at::kBFloat16, at::kFloat}, cap, w, kRead);
   const Mat my = mat(y, "y", {at::kBFloat16}, cap, w, kWrite);
-  std::vector<Mat> others{mx};
+  a.gamma = vec(gamma, "gamma", dim);
+  std::vector<Mat> others{mx, line(const_cast<float*>(a.gamma), dim, "gamma")};
   a.x = mx.p;
   a.f32 = f32(x);
   a.ldx = mx.ld;
@@ -177,6 +189,7 @@ void rmsnorm_fwd(Tensor x, int64_t dim, OptT n_dev, int64_t cap, Tensor gamma, d
     a.s_out = ms.p;
     a.lds = ms.ld;
     apart(ms, mx, true);
+    apart(ms, others[1]);
     apart(ms, mr, true);
   }
   std::vector<Mat> coded;
@@ -189,12 +202,16 @@ void rmsnorm_fwd(Tensor x, int64_t dim, OptT n_dev, int64_t cap, Tensor gamma, d
     apart(m, my);
   }
   if (coded.size() == 2) apart(coded[0], coded[1]);
-  a.gamma = vec(gamma, "gamma", dim);
   a.eps = static_cast<float>(eps);
   TORCH_CHECK(a.eps >= 0.f, "eps must not be negative");
   a.y = my.as<__nv_bfloat16>();
   a.ldy = my.ld;
   a.rstd = vec(rstd, "rstd", cap);
+  const Mat mstd = line(a.rstd, cap, "rstd");
+  all_apart(mstd, others);
+  all_apart(mstd, coded);
+  apart(mstd, ms);
+  apart(mstd, my);
   a.n_ptr = count(n_dev, "n_dev");
   const auto dev = on_device({&x, &gamma, &y, &rstd}, {&n_dev, &residual, &s_out, &q, &q_exp});
   c10::cuda::CUDAGuard g(dev);
@@ -246,6 +263,14 @@ void rmsnorm_bwd(Tensor dy, OptT x, Tensor rstd, Tensor gamma, int64_t dim, OptT
   a.rstd = vec(rstd, "rstd", cap);
   a.gamma = vec(gamma, "gamma", dim);
   a.dgamma = vec(dgamma, "dgamma", dim);
+  const Mat mgam = line(a.dgamma, dim, "dgamma");
+  all_apart(mgam, others);
+  apart(mgam, my);
+  apart(mgam, mr);
+  apart(mgam, md);
+  apart(mgam, line(const_cast<float*>(a.rstd), cap, "rstd"));
+  apart(md, line(const_cast<float*>(a.rstd), cap, "rstd"));
+  apart(md, line(const_cast<float*>(a.gamma), dim, "gamma"));
   a.accumulate = accumulate;
   a.n_ptr = count(n_dev, "n_dev");
   const auto dev = on_device({&dy, &rstd, &gamma, &dx, &dgamma}, {&x, &n_dev, &dres, &n_res_dev, &q, &q_exp});
@@ -277,7 +302,10 @@ void linear_fwd(Tensor A, Tensor W, OptT n_dev, int64_t cap, Tensor out, Tensor 
   a.ldo = mo.ld;
   TORCH_CHECK(act >= 0 && act <= 3, "act must be 0 (none), 1 (ReLU), 2 (GELU) or 3 (SiLU)");
   a.act = static_cast<int32_t>(act);
-  if (has(bias)) a.bias = vec(*bias, "bias", N);
+  if (has(bias)) {
+    a.bias = vec(*bias, "bias", N);
+    others.push_back(line(const_cast<float*>(a.bias), N, "bias"));
+  }
   Mat mr, mz;
   if (has(residual)) {
     mr = mat(*residual, "residual", {at::kBFloat16}, cap, up(N, 8), kReadTma);
@@ -348,7 +376,13 @@ void linear_act_bwd(Tensor dout, int64_t dim, OptT n_dev, int64_t cap, int64_t a
   a.dropout_salt = static_cast<uint32_t>(salt);
   a.ld_mask = ld_mask.has_value() ? *ld_mask : md.ld;
   TORCH_CHECK(a.ld_mask >= 0, "ld_mask must not be negative");
-  if (has(dbias)) a.dbias = vec(*dbias, "dbias", dim);
+  if (has(dbias)) {
+    a.dbias = vec(*dbias, "dbias", dim);
+    const Mat mb = line(a.dbias, dim, "dbias");
+    all_apart(mb, others);
+    apart(mb, mg);
+    apart(mb, md);
+  }
   a.accumulate = accumulate;
   a.n_ptr = count(n_dev, "n_dev");
   const auto dev = on_device({&dout, &dz}, {&n_dev, &dbias, &z, &q, &q_exp, &counters});
